@@ -252,6 +252,105 @@ int axf_hip_add(axf_ctx* ctx, float* y, const float* a, const float* b, int n);
 int axf_hip_embed(axf_ctx* ctx, float* out, int qtype, const void* W, int token, int rows,
                   int cols);
 
+/* ---- several continuations of a text: a cache in pages ---------------------
+ * No reference counterpart: the reference decodes one sequence over one cache.
+ * Beam search and drafted (speculated) token trees keep many continuations at
+ * once; their K/V rows live in pages that continuations share.
+ *
+ * A page holds page_rows consecutive positions' rows of n_kv_heads * head_dim
+ * values (the decoder's cache row).  Row r of page p of layer l is at row
+ * (l * n_pages + p) * page_rows + r of k and of v.  A sequence's position j is
+ * row j % page_rows of page table[j / page_rows]; tables are device int32 rows
+ * of table_ld entries, one row a sequence.  An entry outside 0..n_pages-1 (-1 by
+ * convention) holds no rows: reads see nothing there and writes are dropped.
+ * type: AXF_TYPE_F32 or AXF_TYPE_F16; page_rows: a power of two up to 1024;
+ * head_dim 64, 128 or 256; k and v 16-byte aligned.  Integer arrays (table, len,
+ * n_tok, pos, ...) are device memory, so that a step needs no host round trip. */
+typedef struct {
+    void* k;
+    void* v;
+    int type;
+    int n_layers, n_pages, page_rows, n_kv_heads, head_dim;
+} axf_kv_pages;
+
+/* Host: a drafted tree's masks and depths for axf_hip_attn_paged.  Node i
+ * follows node parent[i] (-1: the text itself; parent[i] < i); bit j of mask[i] is
+ * set where node i sees node j: itself and its ancestors.  depth[i] (may be
+ * NULL) is its distance from the text's next position.  n <= 64. */
+int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n);
+
+/* New sequences from old ones (beams stepping on, drafts cut back, sequences
+ * ending): output sequence i continues input sequence parent[i] with its first
+ * len[i] rows and room for `extra` rows more.
+ *   - Full pages are shared; refs counts each page's holders (tables' entries).
+ *   - With extra > 0 the page that len[i] ends in must be its own: the first of
+ *     the outputs (lowest i) that need a page keeps it if nothing else holds it,
+ *     the others get a copy of its first len[i] % page_rows rows, in all layers.
+ *   - Pages for the rest of the room are taken from those that nothing holds,
+ *     lowest first, in the order of (i, position); when none is left the entry
+ *     is -1.  What the input tables held and no output holds is free again.
+ *   - parent[i] outside 0..n_in-1 or len[i] < 0: sequence i holds nothing.
+ * A text starts as an input row of -1 with len 0.  table_out: n_out rows of
+ * table_ld entries, entries past the room -1, not the array `table`.  refs_out
+ * (n_pages) may be refs.  info (3 int32): copied pages, entries left without a
+ * page, pages free afterwards.  Room past table_ld pages is cut off there. */
+int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, int32_t* refs_out,
+                    int32_t* info, const int32_t* table, const int32_t* refs, int n_in,
+                    const int32_t* parent, const int32_t* len, int n_out, int table_ld, int extra);
+
+/* K and V rows of new tokens into their pages, rounded to the pages' type: row
+ * (s, i) for i < n_tok[s] (n_tok may be NULL: max_tok) goes to position
+ * len[s] + i of sequence s.  K row at k + (s * max_tok + i) * k_ld, plus bk, turned
+ * (rotate-half RoPE) by row pos[s * max_tok + i] of the tables (cos_t/sin_t
+ * [n_pos][head_dim/2], pos clamped to them); pos NULL: not turned.  V row plus
+ * bv.  bk, bv may be NULL. */
+int axf_hip_kv_store(axf_ctx* ctx, const axf_kv_pages* kv, int layer, const int32_t* table,
+                     int table_ld, const int32_t* len, const int32_t* n_tok, int n_seq,
+                     int max_tok, const float* k, int k_ld, const float* bk, const float* v,
+                     int v_ld, const float* bv, const int32_t* pos, const float* cos_t,
+                     const float* sin_t, int n_pos);
+
+/* Attention of n_tok[s] <= max_tok tokens a sequence (NULL: max_tok, at most 64)
+ * over the sequence's len[s] cached rows and the tokens' own rows, which are at
+ * positions len[s] .. len[s] + n_tok[s] - 1 (axf_hip_kv_store).  Token i sees all
+ * len[s] rows and own row j where bit j of mask[s * max_tok + i] is set (j <
+ * n_tok[s]); mask NULL: j <= i.  One token a sequence is a decode step, a mask
+ * a drafted tree, NULL several tokens of one continuation.  q row (s, i) at
+ * q + (s * max_tok + i) * q_ld plus bq (may be NULL), turned by pos as in
+ * axf_hip_kv_store (pos NULL: already turned).  out row (s, i) of n_heads *
+ * head_dim floats, outq8 (may be NULL) its Q8_0 blocks; a row that sees nothing
+ * is zero, rows i >= n_tok[s] are left as they were.  What a masked place holds
+ * (NaN and infinities too) changes nothing.  max_len: about the longest len[s],
+ * for the split of the work; any value gives the same sums up to their order. */
+int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, int q_ld,
+                       const float* bq, const axf_kv_pages* kv, int layer, const int32_t* table,
+                       int table_ld, const int32_t* len, const int32_t* n_tok,
+                       const uint64_t* mask, const int32_t* pos, const float* cos_t,
+                       const float* sin_t, int n_pos, int n_seq, int max_tok, int max_len,
+                       int n_heads);
+
+/* After a drafted tree was verified: rows len[s] + path[s * max_path + i] move to
+ * len[s] + i for i < n_path[s], in all layers, and len_out[s] = len[s] + n_path[s]
+ * (len_out may be len).  A path ascends (0 <= path[0] < path[1] < ...), as a
+ * tree's ways down do; it ends before an entry that does not.  max_path <= 64. */
+int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
+                       const int32_t* table, int table_ld, const int32_t* len,
+                       const int32_t* path, const int32_t* n_path, int n_seq, int max_path);
+
+/* Beam search's selection: of all continuations of n_beams beams a sequence the
+ * n_out best.  Beam b of sequence s has logits row s * n_beams + b (ld floats
+ * apart) and the score cum[s * n_beams + b]; its continuation by token t scores
+ * cum + (x[t] - log sum exp x), in 64 bits.  They rank by score, then lower
+ * beam, higher logit, lower token.  done (may be NULL): a beam with done != 0 has
+ * one continuation, eos_id, that keeps its score.  A score of -inf or NaN (a
+ * masked token, an unused beam with cum -inf; a row with a NaN or +inf logit) is
+ * no continuation.  token, parent (the beam, 0..n_beams-1) and score: n_out a
+ * sequence, best first; -1, -1 and -inf where there are no more.  n_beams and
+ * n_out up to 64, n_vocab up to 2^26. */
+int axf_hip_beam_select(axf_ctx* ctx, int32_t* token, int32_t* parent, float* score,
+                        const float* logits, int ld, const float* cum, const int32_t* done,
+                        int eos_id, int n_seq, int n_beams, int n_vocab, int n_out);
+
 /* ---- timing (stream-ordered HIP events on the context stream) ----------- */
 int axf_hip_timer_start(axf_ctx* ctx);
 int axf_hip_timer_stop(axf_ctx* ctx, float* ms); /* waits for the stop event */

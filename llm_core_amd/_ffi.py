@@ -66,6 +66,19 @@ class Sampling(C.Structure):
     ]
 
 
+class KvPages(C.Structure):
+    _fields_ = [
+        ("k", C.c_void_p),
+        ("v", C.c_void_p),
+        ("type", C.c_int),
+        ("n_layers", C.c_int),
+        ("n_pages", C.c_int),
+        ("page_rows", C.c_int),
+        ("n_kv_heads", C.c_int),
+        ("head_dim", C.c_int),
+    ]
+
+
 class GgufTensor(C.Structure):
     _fields_ = [
         ("name", C.c_char_p),
@@ -150,6 +163,14 @@ SIGNATURES: dict[str, list] = {
     "axf_hip_swiglu": [vp, vp, vp, vp, vp, i32],
     "axf_hip_add": [vp, vp, vp, vp, i32],
     "axf_hip_embed": [vp, vp, i32, vp, i32, i32, i32],
+    "axf_tree_masks": [vp, vp, vp, i32],
+    "axf_hip_kv_fork": [vp, C.POINTER(KvPages), vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32],
+    "axf_hip_kv_store": [vp, C.POINTER(KvPages), i32, vp, i32, vp, vp, i32, i32, vp, i32, vp, vp,
+                         i32, vp, vp, vp, vp, i32],
+    "axf_hip_attn_paged": [vp, vp, vp, vp, i32, vp, C.POINTER(KvPages), i32, vp, i32, vp, vp, vp,
+                           vp, vp, vp, i32, i32, i32, i32, i32],
+    "axf_hip_kv_compact": [vp, C.POINTER(KvPages), vp, vp, i32, vp, vp, vp, i32, i32],
+    "axf_hip_beam_select": [vp, vp, vp, vp, vp, i32, vp, vp, i32, i32, i32, i32, i32],
     "axf_hip_timer_start": [vp],
     "axf_hip_timer_stop": [vp, C.POINTER(f32)],
     "axf_hip_bench_gemv": [vp, i32, vp, C.POINTER(vp), i32, vp, i32, i32, sz, i32, C.POINTER(f32)],

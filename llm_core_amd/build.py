@@ -38,7 +38,10 @@ SOURCES = [
     "kernels/attention.hip",
     "kernels/sample.hip",
     "kernels/gemv_misc.hip",
+    "kernels/paged.hip",
+    "kernels/beam.hip",
     "capi.cpp",
+    "capi_paged.cpp",
     "gemm_noalloc.cpp",
     "host/synth.cpp",
     "host/llama_hip.cpp",

@@ -1,5 +1,5 @@
 // capi.cpp — C-ABI entry points of libaxf_hip.so (declared in include/axf_hip.h).
-#include "capi_internal.hpp"
+#include "capi_check.hpp"
 
 #include <cmath>
 #include <cstdio>
@@ -36,20 +36,6 @@ int ctx_scratch(axf_ctx* ctx, size_t bytes, void** p) {
 }  // namespace axf
 
 using namespace axf;
-
-#define AXF_CHECK_CTX(ctx) \
-    if (!(ctx)) return fail(AXF_ERR_INVALID_ARG, std::string(__func__) + ": null context")
-#define AXF_REQUIRE(cond, msg) \
-    if (!(cond)) return fail(AXF_ERR_INVALID_ARG, std::string(__func__) + ": " + (msg))
-#define AXF_HIP(call)                                          \
-    do {                                                       \
-        hipError_t e_ = (call);                                \
-        if (e_ != hipSuccess) return hip_fail(e_, __func__);   \
-    } while (0)
-
-static inline bool aligned(const void* p, size_t a) {
-    return (reinterpret_cast<uintptr_t>(p) % a) == 0;
-}
 
 extern "C" {
 

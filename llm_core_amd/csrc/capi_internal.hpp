@@ -320,4 +320,61 @@ inline int sample_k(const axf_sampling& s, int n_vocab) {
     return (s.top_k > 0 && s.top_k < n_vocab) ? s.top_k : n_vocab;
 }
 
+// A cache in pages and beam search (kernels/paged.hip, kernels/beam.hip).  Rows of
+// token (s, i) are s * max_tok + i; table / len / n_tok / pos / mask on the device.
+struct PagedArgs {
+    const float* q;
+    int q_ld;
+    const float* bq;
+    const void* k;  // layer's first page
+    const void* v;
+    const int* table;
+    int table_ld;
+    const int* len;
+    const int* n_tok;      // nullptr: max_tok
+    const uint64_t* mask;  // nullptr: causal among the tokens
+    const int* pos;        // nullptr: q is turned already
+    const float *cos_t, *sin_t;
+    int n_pos, n_seq, max_tok, n_heads, n_kv_heads;
+    int n_pages, page_shift;
+    int nsplit, split_rows;  // split j: positions [j * split_rows, ...), the last one to the end
+    float* part;             // [row][head][nsplit][HD + 2]: m (base 2), l, o
+    float* out;
+    uint8_t* outq8;
+};
+void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len);
+size_t attn_paged_scratch(const PagedArgs& a, int head_dim);
+hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, hipStream_t st);
+struct KvStoreArgs {
+    void *k, *v;  // layer's first page
+    const int* table;
+    int table_ld;
+    const int *len, *n_tok, *pos;
+    const float *xk, *xv, *bk, *bv, *cos_t, *sin_t;
+    int k_ld, v_ld, n_pos, n_seq, max_tok, n_kv_heads, n_pages, page_shift;
+};
+hipError_t launch_kv_store(const KvStoreArgs& a, int kv_type, int head_dim, hipStream_t st);
+struct KvForkArgs {
+    int *table_out, *refs_out, *info;
+    const int *table, *refs, *parent, *len;
+    int n_in, n_out, table_ld, extra, n_pages, page_shift;
+    int* scratch;  // kv_fork_scratch() bytes
+};
+size_t kv_fork_scratch(int n_pages, int n_out);
+hipError_t launch_kv_fork(const KvForkArgs& a, const axf_kv_pages& kv, hipStream_t st);
+hipError_t launch_kv_compact(const axf_kv_pages& kv, int* len_out, const int* table, int table_ld,
+                             const int* len, const int* path, const int* n_path, int n_seq,
+                             int max_path, hipStream_t st);
+struct BeamArgs {
+    int *token, *parent;
+    float* score;
+    const float* logits;
+    const float* cum;
+    const int* done;
+    int ld, eos, n_seq, n_beams, n_vocab, n_out;
+    void* scratch;  // beam_scratch() bytes
+};
+size_t beam_scratch(const BeamArgs& a);
+hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st);
+
 }  // namespace axf

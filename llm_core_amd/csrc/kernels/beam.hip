@@ -1,0 +1,350 @@
+// beam.hip — beam search's selection: the best continuations of a sequence's beams
+// over the vocabulary (axf_hip_beam_select).
+//
+//   score(b, t) = cum[b] + (x[b][t] - lse[b]),  lse[b] = log sum_t exp x[b][t]
+//
+// Which of two continuations is better may hang on the last bits of a score, so
+// exponentials, sums and scores are 64-bit (the fp64 units run at the fp32 rate
+// here, and a logit costs some 20 operations against 4 bytes from HBM).  Within a
+// beam the score rises with the logit, so one pass over the logits suffices:
+//   1. k_beam_part: a workgroup takes a chunk of a row: its maximum m, sum of
+//      exp(x - m) and its n_out largest (logit, lower token first) keys.
+//   2. k_beam_merge: a workgroup a sequence joins the chunks' sums to each beam's
+//      lse, turns the keys into scores and merges the chunks' sorted lists to
+//      the n_out best.
+#include "common.hpp"
+
+namespace axf {
+
+namespace {
+
+constexpr int kMergeThreads = 1024;
+
+__device__ __forceinline__ uint32_t ordered32(float v) {
+    const uint32_t u = __float_as_uint(v + 0.f);  // -0 and +0 are one logit
+    return u ^ ((uint32_t)((int32_t)u >> 31) | 0x80000000u);
+}
+__device__ __forceinline__ float unordered32(uint32_t o) {
+    return __uint_as_float((o & 0x80000000u) ? (o ^ 0x80000000u) : ~o);
+}
+__device__ __forceinline__ uint64_t ordered64(double v) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v + 0.0);
+    return u ^ ((uint64_t)((int64_t)u >> 63) | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double unordered64(uint64_t o) {
+    return __longlong_as_double((int64_t)((o >> 63) ? (o ^ 0x8000000000000000ull) : ~o));
+}
+
+// exp(x) for x <= 0 to 2e-13 of its value: 2^k times the Taylor polynomial of
+// degree 10 on [-ln2/2, ln2/2] (its first term left out: 0.347^11 / 11! = 2.2e-13).
+// Below -708 zero; NaN stays NaN.
+__device__ __forceinline__ double exp_neg(double x) {
+    const double k = __builtin_rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(k, -6.93147180369123816490e-01, x);  // ln 2 in two parts
+    r = __builtin_fma(k, -1.90821492927058770002e-10, r);
+    double p = 1.0 / 3628800;
+    p = __builtin_fma(p, r, 1.0 / 362880);
+    p = __builtin_fma(p, r, 1.0 / 40320);
+    p = __builtin_fma(p, r, 1.0 / 5040);
+    p = __builtin_fma(p, r, 1.0 / 720);
+    p = __builtin_fma(p, r, 1.0 / 120);
+    p = __builtin_fma(p, r, 1.0 / 24);
+    p = __builtin_fma(p, r, 1.0 / 6);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    const int e = (int)fmax(k, -1022.0);
+    const double y = __builtin_ldexp(p, e);
+    return x < -708.0 ? 0.0 : y;
+}
+
+__device__ __forceinline__ double wave_sum64(double v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off, 64);
+    return v;
+}
+
+// The k-th largest of the wave's 64 keys (k >= 1; keys differ unless 0): bit by
+// bit from the top, the largest value that at least k keys reach.
+__device__ __forceinline__ uint64_t kth_of_wave(uint64_t key, int k) {
+    const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
+    uint32_t t = 0;
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t c = t | (1u << b);
+        if (__popcll(__ballot(hi >= c)) >= k) t = c;
+    }
+    const int above = __popcll(__ballot(hi > t));
+    const bool same = hi == t;
+    if (__popcll(__ballot(same)) == k - above) {  // all of the equal ones: their least
+        uint32_t u = same ? lo : 0xffffffffu;
+#pragma unroll
+        for (int off = 32; off > 0; off >>= 1) u = min(u, (uint32_t)__shfl_xor((int)u, off, 64));
+        return ((uint64_t)t << 32) | u;
+    }
+    uint32_t v = 0;
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t c = v | (1u << b);
+        if (__popcll(__ballot(same && lo >= c)) >= k - above) v = c;
+    }
+    return ((uint64_t)t << 32) | v;
+}
+
+constexpr int kCap = 512;  // keys ranked at once
+
+// Chunk blockIdx.x of row blockIdx.y: keys[n_out] (largest first, 0: none), m, s.
+// Thread t holds elements 4 (t + NT j) .. +3, j < V4, of the chunk: the same ones
+// whatever the row's alignment.  Every thread's largest key is known without a
+// sort; the n_out-th largest of a wave's 64 is a bound that n_out keys reach, and
+// the keys that reach the largest such bound (some n_out to 3 n_out of them) are
+// ranked by counting.
+template <int NT, int V4>
+__global__ __launch_bounds__(NT) void k_beam_part(const float* __restrict__ logits, int ld, int n_vocab,
+                                                  int n_out, int vec, uint64_t* __restrict__ keys,
+                                                  float* __restrict__ ms, double* __restrict__ ss) {
+    constexpr int NW = NT / 64, CH = NT * V4 * 4;
+    __shared__ uint64_t list[kCap];
+    __shared__ uint64_t bound[NW];
+    __shared__ float wm[NW];
+    __shared__ double wsum[NW];
+    __shared__ int count;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const float* x = logits + (size_t)blockIdx.y * ld;
+    const int base = blockIdx.x * CH;
+    float v[V4 * 4];
+#pragma unroll
+    for (int j = 0; j < V4; j++) {
+        const int i = base + 4 * (t + NT * j);
+        if (vec && i + 3 < n_vocab) {
+            const float4 f = *reinterpret_cast<const float4*>(x + i);
+            v[4 * j] = f.x;
+            v[4 * j + 1] = f.y;
+            v[4 * j + 2] = f.z;
+            v[4 * j + 3] = f.w;
+        } else {
+#pragma unroll
+            for (int e = 0; e < 4; e++) v[4 * j + e] = i + e < n_vocab ? x[i + e] : -INFINITY;
+        }
+    }
+    auto key_of = [&](int j, int e) {
+        const int i = base + 4 * (t + NT * j) + e;
+        return i < n_vocab ? ((uint64_t)ordered32(v[4 * j + e]) << 32) | (uint32_t)~i : 0ull;
+    };
+    uint64_t best = 0;
+    float m = -INFINITY;
+#pragma unroll
+    for (int j = 0; j < V4; j++) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const uint64_t k = key_of(j, e);
+            best = k > best ? k : best;
+            m = fmaxf(m, v[4 * j + e]);
+        }
+    }
+    m = wave_max(m);
+    const uint64_t mine = kth_of_wave(best, n_out);
+    if (lane == 0) {
+        bound[wave] = mine;
+        wm[wave] = m;
+    }
+    if (t == 0) count = 0;
+    __syncthreads();
+    uint64_t least = bound[0];
+    m = wm[0];
+#pragma unroll
+    for (int w = 1; w < NW; w++) {
+        least = bound[w] > least ? bound[w] : least;
+        m = fmaxf(m, wm[w]);
+    }
+    least = least ? least : 1;  // 0: no element
+    // the keys that reach the bound
+    int reach = 0;
+#pragma unroll
+    for (int j = 0; j < V4; j++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) reach += key_of(j, e) >= least;
+    const int at = reach ? atomicAdd(&count, reach) : 0;
+    __syncthreads();
+    int n = count;
+    if (n > kCap) {
+        // few threads hold many large keys: the n_out-th largest of all, bit by bit
+        uint64_t c = 0;
+        for (int b = 63; b >= 0; b--) {
+            const uint64_t probe = c | (1ull << b);
+            int r = 0;
+#pragma unroll
+            for (int j = 0; j < V4; j++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) r += key_of(j, e) >= probe;
+            __syncthreads();
+            if (t == 0) count = 0;
+            __syncthreads();
+            if (r) atomicAdd(&count, r);
+            __syncthreads();
+            if (count >= n_out) c = probe;
+        }
+        least = c ? c : 1;
+        reach = 0;
+#pragma unroll
+        for (int j = 0; j < V4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) reach += key_of(j, e) >= least;
+        __syncthreads();
+        if (t == 0) count = 0;
+        __syncthreads();
+        int o = reach ? atomicAdd(&count, reach) : 0;
+        if (reach)
+            for (int j = 0; j < V4; j++)
+                for (int e = 0; e < 4; e++)
+                    if (key_of(j, e) >= least) list[o++] = key_of(j, e);
+        __syncthreads();
+        n = count;
+    } else if (reach) {
+        int o = at;
+#pragma unroll
+        for (int j = 0; j < V4; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (key_of(j, e) >= least) list[o++] = key_of(j, e);
+    }
+    // sum of exponentials; a NaN or +inf logit makes it NaN, as it does the row's
+    const double top = m == -INFINITY ? 0.0 : (double)m;
+    double s = 0.0;
+#pragma unroll
+    for (int j = 0; j < V4 * 4; j++) s += exp_neg((double)v[j] - top);
+    s = wave_sum64(s);
+    if (lane == 0) wsum[wave] = s;
+    __syncthreads();
+    const size_t chunk = (size_t)blockIdx.y * gridDim.x + blockIdx.x;
+    if (t == 0) {
+        double sum = wsum[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) sum += wsum[w];
+        ss[chunk] = sum;
+        ms[chunk] = m;
+    }
+    uint64_t* out = keys + chunk * n_out;
+    for (int c = t; c < n; c += NT) {
+        const uint64_t k = list[c];
+        int rank = 0;
+        for (int j = 0; j < n; j++) rank += list[j] > k;
+        if (rank < n_out) out[rank] = k;
+    }
+    for (int c = n + t; c < n_out; c += NT) out[c] = 0;
+}
+
+// A continuation: score, and what breaks ties (beam, logit, token), both larger for
+// the better; score 0: none.
+struct Cand {
+    uint64_t score, tie;
+};
+__device__ __forceinline__ bool better(const Cand& a, const Cand& b) {
+    return a.score > b.score || (a.score == b.score && a.tie > b.tie);
+}
+__device__ __forceinline__ Cand lane_xor(const Cand& c, int x) {
+    return {__shfl_xor(c.score, x, 64), __shfl_xor(c.tie, x, 64)};
+}
+
+// a and b: descending lists over the wave's lanes.  The 64 best of both, descending:
+// the better of a[i] and b[63 - i] are a bitonic list of them, sorted in 6 steps.
+__device__ __forceinline__ Cand merge64(Cand a, Cand b) {
+    const int lane = threadIdx.x & 63;
+    const Cand r = lane_xor(b, 63);
+    a = better(r, a) ? r : a;
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) {
+        const Cand o = lane_xor(a, off);
+        const bool keep_max = (lane & off) == 0;
+        a = (better(o, a) == keep_max) ? o : a;
+    }
+    return a;
+}
+
+__global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
+    BeamArgs a, int chunks, const uint64_t* __restrict__ keys, const float* __restrict__ ms,
+    const double* __restrict__ ss) {
+    constexpr int NW = kMergeThreads / 64;
+    __shared__ double lse[64];
+    __shared__ Cand half[NW / 2][64];
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const size_t row0 = (size_t)blockIdx.x * a.n_beams;
+    for (int b = wave; b < a.n_beams; b += NW) {
+        const float* mr = ms + (row0 + b) * chunks;
+        const double* sr = ss + (row0 + b) * chunks;
+        float m = -INFINITY;
+        for (int c = lane; c < chunks; c += 64) m = fmaxf(m, mr[c]);
+        m = wave_max(m);
+        const double top = m == -INFINITY ? 0.0 : (double)m;
+        double s = 0.0;
+        for (int c = lane; c < chunks; c += 64) s += sr[c] * exp_neg((double)mr[c] - top);
+        s = wave_sum64(s);
+        // all logits -inf: log 0, and every score -inf - -inf
+        if (lane == 0) lse[b] = top + log(s);
+    }
+    __syncthreads();
+    Cand acc = {0, 0};
+    for (int l = wave; l < a.n_beams * chunks; l += NW) {
+        const int b = l / chunks;
+        const bool over = a.done && a.done[row0 + b] != 0;
+        Cand c = {0, 0};
+        const double cum = (double)a.cum[row0 + b];
+        if (over) {
+            if (l % chunks == 0 && lane == 0 && cum > -INFINITY)
+                c = {ordered64(cum), ((uint64_t)(63 - b) << 58) | (uint64_t)(0x3ffffff - a.eos)};
+        } else if (lane < a.n_out) {
+            const uint64_t k = keys[(row0 * chunks + l) * a.n_out + lane];
+            const uint32_t x = (uint32_t)(k >> 32);
+            const double score = cum + ((double)unordered32(x) - lse[b]);
+            if (k && score > -INFINITY)
+                c = {ordered64(score), ((uint64_t)(63 - b) << 58) | ((uint64_t)x << 26) |
+                                           (uint64_t)(0x3ffffff - ~(uint32_t)k)};
+        }
+        acc = l == wave ? c : merge64(acc, c);
+    }
+    for (int n = NW / 2; n > 0; n >>= 1) {
+        if (wave >= n && wave < 2 * n) half[wave - n][lane] = acc;
+        __syncthreads();
+        if (wave < n) acc = merge64(acc, half[wave][lane]);
+        __syncthreads();
+    }
+    if (wave == 0 && lane < a.n_out) {
+        const size_t o = (size_t)blockIdx.x * a.n_out + lane;
+        const bool none = acc.score == 0;
+        a.token[o] = none ? -1 : 0x3ffffff - (int)(acc.tie & 0x3ffffff);
+        a.parent[o] = none ? -1 : 63 - (int)(acc.tie >> 58);
+        a.score[o] = none ? -INFINITY : (float)unordered64(acc.score);
+    }
+}
+
+constexpr int kPartThreads = 256;
+constexpr int kChunk = kPartThreads * 4 * 2;
+
+}  // namespace
+
+static int beam_chunks(const BeamArgs& a) { return (a.n_vocab + kChunk - 1) / kChunk; }
+
+size_t beam_scratch(const BeamArgs& a) {
+    const size_t lists = (size_t)a.n_seq * a.n_beams * beam_chunks(a);
+    return lists * (8 * a.n_out + 8 + 4);
+}
+
+hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st) {
+    const int chunks = beam_chunks(a);
+    const size_t lists = (size_t)a.n_seq * a.n_beams * chunks;
+    uint64_t* keys = static_cast<uint64_t*>(a.scratch);
+    double* ss = reinterpret_cast<double*>(keys + lists * a.n_out);
+    float* ms = reinterpret_cast<float*>(ss + lists);
+    const int vec = a.ld % 4 == 0 && (reinterpret_cast<uintptr_t>(a.logits) & 15) == 0;
+    const long rows = (long)a.n_seq * a.n_beams;
+    // grid.y holds 65535 rows
+    for (long r = 0; r < rows; r += 65535) {
+        const unsigned n = (unsigned)(rows - r < 65535 ? rows - r : 65535);
+        const size_t at = (size_t)r * chunks;
+        k_beam_part<kPartThreads, 2><<<dim3(chunks, n), kPartThreads, 0, st>>>(
+            a.logits + (size_t)r * a.ld, a.ld, a.n_vocab, a.n_out, vec, keys + at * a.n_out, ms + at,
+            ss + at);
+    }
+    k_beam_merge<<<a.n_seq, kMergeThreads, 0, st>>>(a, chunks, keys, ms, ss);
+    return hipGetLastError();
+}
+
+}  // namespace axf

@@ -48,6 +48,24 @@ class Buffer:
         return self.ptr
 
 
+class KvPages:
+    """A cache in pages (axf_kv_pages): K and V pools of [n_layers][n_pages][page_rows]
+    rows of n_kv_heads * head_dim values of GGML type `kv_type` (F32 or F16), at device
+    addresses k and v."""
+
+    def __init__(self, k: int, v: int, kv_type: int, n_layers: int, n_pages: int, page_rows: int,
+                 n_kv_heads: int, head_dim: int):
+        self.c = _ffi.KvPages(int(k), int(v), kv_type, n_layers, n_pages, page_rows, n_kv_heads,
+                              head_dim)
+        self.row = n_kv_heads * head_dim
+        self.ref = C.byref(self.c)
+
+
+def _at(p) -> int | None:
+    """A device address argument: None (or 0) is NULL."""
+    return int(p) if p else None
+
+
 class Context:
     def __init__(self, device: int = 0):
         h = C.c_void_p()
@@ -189,6 +207,47 @@ class Context:
         call("axf_hip_embed", self.handle, C.c_void_p(int(out)), qtype, C.c_void_p(int(W)), token,
              rows, cols)
 
+    # ---- several continuations of a text ---------------------------------------
+    def kv_fork(self, kv: KvPages, table_out: int, refs_out: int, info: int, table: int, refs: int,
+                n_in: int, parent: int, length: int, n_out: int, table_ld: int, extra: int) -> None:
+        """New sequences' page tables from old ones (axf_hip_kv_fork)."""
+        call("axf_hip_kv_fork", self.handle, kv.ref, _at(table_out), _at(refs_out), _at(info),
+             _at(table), _at(refs), n_in, _at(parent), _at(length), n_out, table_ld, extra)
+
+    def kv_store(self, kv: KvPages, layer: int, table: int, table_ld: int, length: int, n_seq: int,
+                 max_tok: int, k: int, v: int, k_ld: int = 0, v_ld: int = 0, n_tok: int | None = None,
+                 bk: int | None = None, bv: int | None = None, pos: int | None = None,
+                 cos_t: int | None = None, sin_t: int | None = None, n_pos: int = 0) -> None:
+        """K and V rows of new tokens into their pages; k_ld / v_ld 0: packed rows."""
+        call("axf_hip_kv_store", self.handle, kv.ref, layer, _at(table), table_ld, _at(length),
+             _at(n_tok), n_seq, max_tok, _at(k), k_ld or kv.row, _at(bk), _at(v), v_ld or kv.row,
+             _at(bv), _at(pos), _at(cos_t), _at(sin_t), n_pos)
+
+    def attn_paged(self, out: int, outq8: int | None, q: int, kv: KvPages, layer: int, table: int,
+                   table_ld: int, length: int, n_seq: int, max_tok: int, max_len: int, n_heads: int,
+                   q_ld: int = 0, bq: int | None = None, n_tok: int | None = None,
+                   mask: int | None = None, pos: int | None = None, cos_t: int | None = None,
+                   sin_t: int | None = None, n_pos: int = 0) -> None:
+        """Attention of up to 64 tokens a sequence over a cache in pages; q_ld 0: packed
+        rows, mask None: each token sees its own earlier ones."""
+        call("axf_hip_attn_paged", self.handle, _at(out), _at(outq8), _at(q),
+             q_ld or n_heads * kv.c.head_dim, _at(bq), kv.ref, layer, _at(table), table_ld,
+             _at(length), _at(n_tok), _at(mask), _at(pos), _at(cos_t), _at(sin_t), n_pos, n_seq,
+             max_tok, max_len, n_heads)
+
+    def kv_compact(self, kv: KvPages, len_out: int, table: int, table_ld: int, length: int,
+                   path: int, n_path: int, n_seq: int, max_path: int) -> None:
+        """A verified tree's accepted rows moved together (axf_hip_kv_compact)."""
+        call("axf_hip_kv_compact", self.handle, kv.ref, _at(len_out), _at(table), table_ld,
+             _at(length), _at(path), _at(n_path), n_seq, max_path)
+
+    def beam_select(self, token: int, parent: int, score: int, logits: int, ld: int, cum: int,
+                    n_seq: int, n_beams: int, n_vocab: int, n_out: int, done: int | None = None,
+                    eos_id: int = -1) -> None:
+        """The n_out best continuations of each sequence's beams (axf_hip_beam_select)."""
+        call("axf_hip_beam_select", self.handle, _at(token), _at(parent), _at(score), _at(logits),
+             ld, _at(cum), _at(done), eos_id, n_seq, n_beams, n_vocab, n_out)
+
     def bench_read(self, bufs, nbytes: int, unroll: int, wgs: int, reps: int) -> float:
         """Milliseconds for reps passes of a plain streaming read over bufs."""
         arr = (C.c_void_p * len(bufs))(*[int(b) for b in bufs])
@@ -236,6 +295,15 @@ def rope_table(head_dim: int, theta: float, max_pos: int) -> tuple[np.ndarray, n
     call("axf_rope_table", c.ctypes.data_as(C.c_void_p), s.ctypes.data_as(C.c_void_p), head_dim,
          C.c_float(theta), max_pos)
     return c, s
+
+
+def tree_masks(parent) -> tuple[np.ndarray, np.ndarray]:
+    """(mask uint64, depth int32) of a drafted tree's nodes from their parents (-1: the text)."""
+    p = np.ascontiguousarray(parent, np.int32)
+    mask, depth = np.empty(p.size, np.uint64), np.empty(p.size, np.int32)
+    call("axf_tree_masks", mask.ctypes.data_as(C.c_void_p), depth.ctypes.data_as(C.c_void_p),
+         p.ctypes.data_as(C.c_void_p), int(p.size))
+    return mask, depth
 
 
 def synth_normal(n: int, seed: int, mean: float = 0.0, std: float = 1.0) -> np.ndarray:
@@ -287,6 +355,7 @@ __all__ = [
     "AXF_TYPE_Q6_K",
     "Buffer",
     "Context",
+    "KvPages",
     "Q8_0_BYTES",
     "device_count",
     "rope_table",
@@ -294,5 +363,6 @@ __all__ = [
     "synth_normal",
     "synth_quantize",
     "synth_weight",
+    "tree_masks",
     "_ffi",
 ]
