@@ -45,69 +45,510 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
     return x;
 }
 
-// ---- attention: one wave a query row ----------------------------------------
-// Partial result of a split: m (the largest score * log2 e / sqrt(HD)), l (sum of
-// 2^(score - m)) and o (the weighted V sum); the combine kernel joins them.
+// ---- attention ------------------------------------------------------------------
+// A sequence's tokens and the query heads of one KV head are rows of one matrix:
+// row rho = i * G + h of token i, head kvh * G + h.  S^T = K Q^T and O^T = V^T P^T on
+// the matrix cores (16x16x32), the softmax online: a running maximum m and sum l a
+// row, in base 2 (t = s * log2(e) / sqrt(HD)).  With the products transposed a lane
+// keeps one query row (its column, lane & 15) through both: S^T leaves it 4 keys of a
+// 16-key tile (4 (lane >> 4) + r), two tiles are the 8 keys that the second product's
+// B operand wants of a lane, so P never leaves its lane, and rescaling O needs no
+// exchange either.
+//
+// fp32 is kept on 16-bit operands by splitting:
+//   F32 pages: x = h + m + l, three bf16 cut off one after the other (exact: 8 bits
+//   each, the whole range of fp32, no scales), and the six products that reach 2^-24
+//   of the largest: hh, hm, mh, mm, hl, lh; 6/16 of the fp32 matrix rate's time.
+//   F16 pages: K and V are fp16 as they are; q (scaled by a power of two a row) and p
+//   are h + 2^-12 l, two fp16 parts with a sum of their own each, 22 bits: two
+//   products and no work on K or V.
+// Infinities and NaN do not split; a wave whose sums end up not finite does its rows
+// again in plain fp32 (row_careful), where each masked place is left out.
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr int kStep = 32;  // keys a step: two 16-key tiles
+
+__device__ __forceinline__ uint32_t pack_hi(float lo, float hi) {
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+__device__ __forceinline__ float cut_bf16(float x) {
+    return __uint_as_float(__float_as_uint(x) & 0xffff0000u);
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+    const _Float16 a = (_Float16)lo, b = (_Float16)hi;
+    uint16_t x, y;
+    __builtin_memcpy(&x, &a, 2);
+    __builtin_memcpy(&y, &b, 2);
+    return (uint32_t)x | ((uint32_t)y << 16);
+}
+
+// How values of a page type become 16-bit operands.  KP / QP: parts of K and V, of q
+// and p; SUMS: accumulators a product needs.
+template <class T>
+struct Parts;
+
+template <>
+struct Parts<float> {
+    static constexpr int KP = 3, QP = 3, SUMS = 1;
+    static __device__ __forceinline__ void split(const float (&x)[8], uint4 (&f)[3]) {
+        uint32_t w[3][4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = x[2 * e], b = x[2 * e + 1];
+            const float a1 = a - cut_bf16(a), b1 = b - cut_bf16(b);
+            const float a2 = a1 - cut_bf16(a1), b2 = b1 - cut_bf16(b1);
+            w[0][e] = pack_hi(a, b);
+            w[1][e] = pack_hi(a1, b1);
+            w[2][e] = pack_hi(a2, b2);
+        }
+#pragma unroll
+        for (int p = 0; p < 3; p++) f[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
+    }
+    static __device__ __forceinline__ void split_q(const float (&x)[8], uint4 (&f)[3]) { split(x, f); }
+    static __device__ __forceinline__ void split_kv(const float (&x)[8], uint4 (&f)[3]) { split(x, f); }
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                       __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    }
+    // the smallest products first
+    static __device__ __forceinline__ void product(const uint4 (&a)[3], const uint4 (&b)[3],
+                                                   f32x4 (&c)[1]) {
+        c[0] = mul(a[2], b[0], c[0]);
+        c[0] = mul(a[0], b[2], c[0]);
+        c[0] = mul(a[1], b[1], c[0]);
+        c[0] = mul(a[1], b[0], c[0]);
+        c[0] = mul(a[0], b[1], c[0]);
+        c[0] = mul(a[0], b[0], c[0]);
+    }
+    static __device__ __forceinline__ float total(const f32x4 (&c)[1], int r) { return c[0][r]; }
+    static constexpr bool kScaleQ = false;
+};
+
+template <>
+struct Parts<_Float16> {
+    static constexpr int KP = 1, QP = 2, SUMS = 2;
+    static __device__ __forceinline__ void split_q(const float (&x)[8], uint4 (&f)[2]) {
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = x[2 * e], b = x[2 * e + 1];
+            const float a0 = (float)(_Float16)a, b0 = (float)(_Float16)b;
+            h[e] = pack_f16(a, b);
+            l[e] = pack_f16((a - a0) * 4096.f, (b - b0) * 4096.f);
+        }
+        f[0] = make_uint4(h[0], h[1], h[2], h[3]);
+        f[1] = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                      __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ void product(const uint4 (&a)[1], const uint4 (&b)[2],
+                                                   f32x4 (&c)[2]) {
+        c[0] = mul(a[0], b[0], c[0]);
+        c[1] = mul(a[0], b[1], c[1]);
+    }
+    static __device__ __forceinline__ float total(const f32x4 (&c)[2], int r) {
+        return fmaf(c[1][r], 1.f / 4096.f, c[0][r]);
+    }
+    static constexpr bool kScaleQ = true;
+};
+
+// Reductions over the four 16-lane rows of a wave (lanes n, n + 16, n + 32, n + 48),
+// every lane receiving the result.  v_permlane{16,32}_swap of a value with itself
+// leaves it beside its partner rows' value.
+__device__ __forceinline__ float rows_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float rows_sum(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// q elements d .. d+7 (d % 8 == 0) of a row: bias and RoPE; zero for no row.
+template <int HD>
+__device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, int d, float (&x)[8]) {
+    auto ld8 = [](const float* p, float (&v)[8]) {
+        const f32x4_a4 u = *reinterpret_cast<const f32x4_a4*>(p);
+        const f32x4_a4 w = *reinterpret_cast<const f32x4_a4*>(p + 4);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            v[e] = u[e];
+            v[4 + e] = w[e];
+        }
+    };
+    const float* qr = a.q + row * a.q_ld + h * HD;
+    ld8(qr + d, x);
+    float b[8];
+    if (a.bq) {
+        ld8(a.bq + h * HD + d, b);
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] += b[e];
+    }
+    if (a.pos) {
+        constexpr int half = HD / 2;
+        const int e2 = d < half ? d + half : d - half, f = d < half ? d : e2;
+        float y[8], c[8], s[8];
+        ld8(qr + e2, y);
+        if (a.bq) {
+            ld8(a.bq + h * HD + e2, b);
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] += b[e];
+        }
+        const long p = min(max(a.pos[row], 0), a.n_pos - 1);
+        ld8(a.cos_t + p * half + f, c);
+        ld8(a.sin_t + p * half + f, s);
+        const float sign = d < half ? -1.f : 1.f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[e] = fmaf(x[e], c[e], sign * (y[e] * s[e]));
+    }
+}
+
+// What a wave needs to know of its sequence and split.
+struct Span {
+    int s, held, tok, j0, j1;
+    const int* table;
+};
+
+__device__ __forceinline__ uint64_t seen_mask(const PagedArgs& a, long row, int i) {
+    return a.mask ? a.mask[row] : ~0ull >> (63 - i);
+}
+
+// One query row in plain fp32, a wave over the head's elements: the steps of 32 keys
+// step0, step0 + stride, ... of the span.  o: elements lane + 64 e.
 template <int HD, class T>
-__global__ __launch_bounds__(256) void k_attn_paged_rows(PagedArgs a) {
+__device__ __noinline__ void row_careful(const PagedArgs& a, const Span& sp, int rho, int kvh, int step0,
+                                         int stride, float& m, float& l, float* o) {
     constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63;
-    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-    const long rows = (long)a.n_seq * a.max_tok * a.n_heads;
-    if (w >= rows) return;
-    const int h = (int)(w % a.n_heads);
-    const long row = w / a.n_heads;
-    const int i = (int)(row % a.max_tok), s = (int)(row / a.max_tok);
-    const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
-    if (i >= n.tok) return;
-    const int total = n.held + n.tok;
-    const int j0 = blockIdx.y * a.split_rows;
-    const int j1 = (int)blockIdx.y + 1 == a.nsplit ? total : min(total, j0 + a.split_rows);
-    const int kvh = h / (a.n_heads / a.n_kv_heads);
-    const int ld = a.n_kv_heads * HD;
-    const uint64_t mask = a.mask ? a.mask[row] : ~0ull >> (63 - i);
-    const int* table = a.table + (long)s * a.table_ld;
+    const int lane = threadIdx.x & 63, G = a.n_heads / a.n_kv_heads;
+    const int i = rho / G, h = kvh * G + rho % G;
+    const long row = (long)sp.s * a.max_tok + i, ld = (long)a.n_kv_heads * HD;
+    const uint64_t mask = seen_mask(a, row, i);
     const T* k = static_cast<const T*>(a.k) + kvh * HD;
     const T* v = static_cast<const T*>(a.v) + kvh * HD;
     const float c = kLog2e / sqrtf((float)HD);
-    float q[E], o[E];
+    float q[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
         q[e] = q_value<HD>(a, row, h, lane + 64 * e);
         o[e] = 0.f;
     }
-    float m = -INFINITY, l = 0.f;
-    for (int j = j0; j < j1; j++) {
-        if (j >= n.held && !((mask >> (j - n.held)) & 1)) continue;
-        const long r = kv_row(j, table, a.table_ld, a.n_pages, a.page_shift);
-        if (r < 0) continue;
-        float d = 0.f;
+    m = -INFINITY;
+    l = 0.f;
+    for (int b = sp.j0 + step0 * kStep; b < sp.j1; b += stride * kStep) {
+        for (int j = b; j < min(b + kStep, sp.j1); j++) {
+            if (j >= sp.held && !((mask >> (j - sp.held)) & 1)) continue;
+            const long r = kv_row(j, sp.table, a.table_ld, a.n_pages, a.page_shift);
+            if (r < 0) continue;
+            float d = 0.f;
 #pragma unroll
-        for (int e = 0; e < E; e++) d = fmaf(q[e], kv_value(k[r * ld + lane + 64 * e]), d);
-        d = wave_sum(d) * c;
-        const float mn = fmaxf(m, d);
-        const float base = mn == -INFINITY ? 0.f : mn;
-        const float keep = exp2f(m - base), p = exp2f(d - base);
-        l = l * keep + p;
+            for (int e = 0; e < E; e++) d = fmaf(q[e], (float)k[r * ld + lane + 64 * e], d);
+            d = wave_sum(d) * c;
+            if (d == -INFINITY) continue;  // no weight, whatever the value
+            const float mn = fmaxf(m, d);
+            const float base = mn == -INFINITY ? 0.f : mn;
+            const float keep = exp2f(m - base), p = exp2f(d - base);
+            l = l * keep + p;
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(p, kv_value(v[r * ld + lane + 64 * e]), o[e] * keep);
-        m = mn;
+            for (int e = 0; e < E; e++)
+                o[e] = fmaf(p, (float)v[r * ld + lane + 64 * e], keep == 0.f ? 0.f : o[e] * keep);
+            m = mn;
+        }
     }
-    if (a.nsplit == 1 && !a.outq8) {
-        float* dst = a.out + row * a.n_heads * HD + h * HD;
-#pragma unroll
-        for (int e = 0; e < E; e++) dst[lane + 64 * e] = l == 0.f ? 0.f : o[e] / l;
-        return;
-    }
-    float* dst = a.part + (w * a.nsplit + blockIdx.y) * (HD + 2);
-    if (lane == 0) {
-        dst[0] = m;
-        dst[1] = l;
-    }
-#pragma unroll
-    for (int e = 0; e < E; e++) dst[2 + lane + 64 * e] = o[e];
 }
 
+// q's fragments of one 16-row tile: lane's row, elements 32 c + 8 (lane >> 4) .. +7 of
+// each 32-element chunk.  scale: what scores are multiplied by (with F16 pages the
+// row was scaled to the top of fp16's range).
+template <int HD, class T>
+__device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, int kvh, bool live,
+                                       uint4 (&qf)[HD / 32][Parts<T>::QP], float& scale) {
+    constexpr int NC = HD / 32;
+    const int g = (threadIdx.x & 63) >> 4, G = a.n_heads / a.n_kv_heads;
+    const int i = rho / G, h = kvh * G + rho % G;
+    float x[NC][8];
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+        if (live) {
+            q_values8<HD>(a, (long)sp.s * a.max_tok + i, h, 32 * c + 8 * g, x[c]);
+        } else {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[c][e] = 0.f;
+        }
+    }
+    scale = kLog2e / sqrtf((float)HD);
+    float up = 1.f;
+    if (Parts<T>::kScaleQ) {
+        float top = 0.f;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][e]));
+        top = rows_max(top);
+        // 2^(14 - exponent): the largest value between 2^14 and 2^15
+        const int ex = top > 0.f ? min(max(14 - (int)__builtin_amdgcn_frexp_expf(top) + 1, -100), 100) : 0;
+        up = __builtin_ldexpf(1.f, ex);
+        scale = __builtin_ldexpf(scale, -ex);
+    }
+#pragma unroll
+    for (int c = 0; c < NC; c++) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) x[c][e] *= up;
+        Parts<T>::split_q(x[c], qf[c]);
+    }
+}
+
+// The weights of one step for the lane's query row from S^T's two tiles: masks,
+// running maximum and sum, and P as the second product's operand.  keep: what O is
+// multiplied by.  bad: bit (4 tile + r) set where the lane's key is no row.
+template <class T>
+__device__ __forceinline__ void weights(const f32x4 (&st)[2][Parts<T>::SUMS], float scale, bool masked,
+                                        uint64_t mask, int jb, const Span& sp, uint32_t bad, float& m,
+                                        float& l, float& keep, uint4 (&pf)[Parts<T>::QP]) {
+    const int g = (threadIdx.x & 63) >> 4;
+    float s[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) s[e] = Parts<T>::total(st[e >> 2], e & 3);
+    if (masked) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int j = jb + 16 * (e >> 2) + 4 * g + (e & 3);
+            const bool own = j >= sp.held;
+            const bool see = j < sp.j1 && !((bad >> e) & 1) &&
+                             (!own || ((mask >> (own ? j - sp.held : 0)) & 1));
+            s[e] = see ? s[e] : -INFINITY;
+        }
+    }
+    float top = s[0];
+#pragma unroll
+    for (int e = 1; e < 8; e++) top = fmaxf(top, s[e]);
+    top = rows_max(top) * scale;
+    const float mn = fmaxf(m, top);
+    const float base = mn == -INFINITY ? 0.f : mn;
+    keep = __builtin_amdgcn_exp2f(m - base);
+    float p[8], sum = 0.f;
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        p[e] = __builtin_amdgcn_exp2f(fmaf(s[e], scale, -base));
+        sum += p[e];
+    }
+    l = fmaf(l, keep, sum);
+    m = mn;
+    Parts<T>::split_q(p, pf);
+}
+
+// ---- up to 16 query rows: a wave needs every K and V value once, so it loads them
+// from memory straight into the operands' layout (K: lane's key row, 8 elements a chunk;
+// V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
+// waves take every fourth step of the split and join at its end.
+constexpr int kFewWaves = 4;
+
+template <int HD, class T>
+__global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, int tiles) {
+    constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
+                  SUMS = Parts<T>::SUMS;
+    __shared__ float os[kFewWaves][16][HD + 4];
+    __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
+    // workgroups of one part of the cache (its row tiles; other sequences' same part,
+    // which may be the same pages) are 8 apart: one XCD's L2 serves them
+    const int per = (a.n_kv_heads * a.nsplit + 7) & ~7;
+    const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
+    const int tile = rest % tiles, c = (rest / tiles) * 8 + xcd;
+    const int x = c % per;
+    if (x >= a.n_kv_heads * a.nsplit) return;
+    const int kvh = x / a.nsplit, split = x % a.nsplit;
+    Span sp;
+    sp.s = c / per;
+    const SeqLen len = seq_len(a.len, a.n_tok, a.max_tok, sp.s, a.table_ld, a.page_shift);
+    sp.held = len.held;
+    sp.tok = len.tok;
+    sp.table = a.table + (long)sp.s * a.table_ld;
+    const int total = sp.held + sp.tok, rows = sp.tok * G;
+    if (tile * 16 >= rows) return;
+    sp.j0 = split * a.split_rows;
+    sp.j1 = split + 1 == a.nsplit ? total : min(total, sp.j0 + a.split_rows);
+    if (sp.j0 >= sp.j1 && split > 0) return;
+    const int rho = tile * 16 + n;
+    const bool live = rho < rows;
+    const long ld = (long)a.n_kv_heads * HD;
+    const T* kb = static_cast<const T*>(a.k) + kvh * HD + 8 * g;
+    const T* vb = static_cast<const T*>(a.v) + kvh * HD + n * ND;
+
+    uint4 qf[NC][QP];
+    float scale;
+    load_q<HD, T>(a, sp, rho, kvh, live, qf, scale);
+    const uint64_t mask = live ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
+    f32x4 o[ND][SUMS];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < SUMS; e++) o[d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    // pool row of the lane's K key of each tile, -1: none
+    auto rows_of = [&](int jb, int (&r)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            r[t] = (int)kv_row(min(jb + 16 * t + n, sp.j1 - 1), sp.table, a.table_ld, a.n_pages,
+                               a.page_shift);
+    };
+    T kr[2][NC][8], vr[2][4][ND];
+    auto load_k = [&](const int (&r)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+            const T* p = kb + (long)max(r[t], 0) * ld;
+#pragma unroll
+            for (int c2 = 0; c2 < NC; c2++)
+                __builtin_memcpy(kr[t][c2], __builtin_assume_aligned(p + 32 * c2, 16), 8 * sizeof(T));
+        }
+    };
+    auto load_v = [&](const int (&r)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int row = __shfl(r[t], 4 * g + e, 64);
+                const T* p = vb + (long)max(row, 0) * ld;
+                __builtin_memcpy(vr[t][e], __builtin_assume_aligned(p, ND * sizeof(T) < 16 ? 8 : 16),
+                                 ND * sizeof(T));
+            }
+    };
+    const int first = sp.j0 + wave * kStep, hop = kFewWaves * kStep;
+    int r[2], rn[2];
+    if (first < sp.j1) {
+        rows_of(first, r);
+        load_k(r);
+        load_v(r);
+    }
+    for (int jb = first; jb < sp.j1; jb += hop) {
+        const bool more = jb + hop < sp.j1;
+        if (more) rows_of(jb + hop, rn);
+        f32x4 st[2][SUMS];
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int e = 0; e < SUMS; e++) st[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int c2 = 0; c2 < NC; c2++) {
+                uint4 kf[KP];
+                if constexpr (KP == 1) {
+                    __builtin_memcpy(&kf[0], kr[t][c2], 16);
+                } else {
+                    Parts<T>::split_kv(kr[t][c2], kf);
+                }
+                Parts<T>::product(kf, qf[c2], st[t]);
+            }
+        }
+        // no row behind a key: only bad tables have such keys before j1
+        const bool hole = __any(r[0] < 0 || r[1] < 0);
+        uint32_t bad = 0;
+        if (hole) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                bad |= (uint32_t)(__shfl(r[e >> 2], 4 * g + (e & 3), 64) < 0) << e;
+        }
+        if (more) load_k(rn);
+        float keep;
+        uint4 pf[QP];
+        weights<T>(st, scale, hole || jb + kStep > min(sp.held, sp.j1), mask, jb, sp, bad, m, l, keep, pf);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+#pragma unroll
+            for (int e = 0; e < SUMS; e++) o[d][e] *= keep;
+            uint4 vf[KP];
+            if constexpr (KP == 1) {
+                T w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = vr[e >> 2][e & 3][d];
+                __builtin_memcpy(&vf[0], w, 16);
+            } else {
+                float w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = vr[e >> 2][e & 3][d];
+                Parts<T>::split_kv(w, vf);
+            }
+            Parts<T>::product(vf, pf, o[d]);
+        }
+        if (more) {
+            load_v(rn);
+            r[0] = rn[0];
+            r[1] = rn[1];
+        }
+    }
+    // the wave's sums, element (4 g + e) * ND + d of row n
+    l = rows_sum(l);
+    float check = l;
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float y = Parts<T>::total(o[d], e);
+            os[wave][n][(4 * g + e) * ND + d] = y;
+            check = fmaf(y, 0.f, check);  // NaN if one of them is not finite
+        }
+    if (g == 0) {
+        ms[wave][n] = m;
+        ls[wave][n] = l;
+    }
+    if (__any(live && !(fabsf(check) < INFINITY))) {
+        for (int t = 0; t < 16 && tile * 16 + t < rows; t++) {
+            float mc, lc, oc[HD / 64];
+            row_careful<HD, T>(a, sp, tile * 16 + t, kvh, wave, kFewWaves, mc, lc, oc);
+            ms[wave][t] = mc;
+            ls[wave][t] = lc;
+#pragma unroll
+            for (int e = 0; e < HD / 64; e++) os[wave][t][lane + 64 * e] = oc[e];
+        }
+    }
+    __syncthreads();
+    // thread: row threadIdx.x / 16, every 16th float4 of it
+    const int t = threadIdx.x >> 4, u = threadIdx.x & 15;
+    if (tile * 16 + t >= rows) return;
+    float top = ms[0][t];
+#pragma unroll
+    for (int w = 1; w < kFewWaves; w++) top = fmaxf(top, ms[w][t]);
+    const float base = top == -INFINITY ? 0.f : top;
+    float f[kFewWaves], sum = 0.f;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; w++) {
+        // a wave without a weight has nothing to add, whatever it holds
+        f[w] = ls[w][t] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[w][t] - base);
+        sum = fmaf(ls[w][t], f[w], sum);
+    }
+    const int ro = tile * 16 + t;
+    const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
+    const bool whole = a.nsplit == 1 && !a.outq8;
+    float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * (HD + 2);
+    if (!whole && u == 0) {
+        dst[0] = top;
+        dst[1] = sum;
+    }
+    const float by = !whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+    for (int d = 4 * u; d < HD; d += 64) {
+        float y[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++) {
+            if (ls[w][t] == 0.f) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = fmaf(os[w][t][d + e], f[w], y[e]);
+        }
+#pragma unroll
+        for (int e = 0; e < 4; e++) dst[(whole ? 0 : 2) + d + e] = y[e] * by;
+    }
+}
+
+// Partial result of a split: m, l (sum of 2^(t - m)) and o (the weighted V sum).
 // One wave a query row and head: the splits' sums brought to one base and added
 // in their order, divided by the weights' sum.
 template <int HD>
@@ -131,6 +572,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a) {
     for (int e = 0; e < E; e++) o[e] = 0.f;
     for (int j = 0; j < used; j++) {
         const float* pj = p + (long)j * (HD + 2);
+        if (pj[1] == 0.f) continue;  // no weight there, whatever it holds
         const float f = exp2f(pj[0] - base);
         l = fmaf(pj[1], f, l);
 #pragma unroll
@@ -439,10 +881,14 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
 
 template <int HD, class T>
 hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
-    const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
-    const unsigned wgs = (unsigned)((waves + 3) / 4);
-    k_attn_paged_rows<HD, T><<<dim3(wgs, a.nsplit), 256, 0, st>>>(a);
-    if (a.nsplit > 1 || a.outq8) k_attn_paged_join<HD><<<wgs, 256, 0, st>>>(a);
+    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads);
+    const int tiles = (rows + 15) / 16;
+    const long per = (a.n_kv_heads * a.nsplit + 7) & ~7;
+    k_attn_paged_few<HD, T><<<(unsigned)(per * a.n_seq * tiles), 64 * kFewWaves, 0, st>>>(a, tiles);
+    if (a.nsplit > 1 || a.outq8) {
+        const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
+        k_attn_paged_join<HD><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
+    }
     return hipGetLastError();
 }
 
@@ -460,9 +906,11 @@ void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     (void)head_dim;
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
-    const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
-    long split = longest * waves / 4096;
-    split = split < 64 ? 64 : (split + 63) / 64 * 64;
+    const long tiles = (a.max_tok * (a.n_heads / a.n_kv_heads) + 15) / 16;
+    const long parts = (long)a.n_seq * a.n_kv_heads * tiles;
+    const long unit = kStep * kFewWaves;
+    long split = longest * parts / 1024;
+    split = split < unit ? unit : (split + unit - 1) / unit * unit;
     a.split_rows = (int)split;
     a.nsplit = (int)((longest + split - 1) / split);
 }
