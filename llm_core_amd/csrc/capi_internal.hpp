@@ -338,7 +338,8 @@ struct PagedArgs {
     int n_pos, n_seq, max_tok, n_heads, n_kv_heads;
     int n_pages, page_shift;
     int nsplit, split_rows;  // split j: positions [j * split_rows, ...), the last one to the end
-    float* part;             // [row][head][nsplit][HD + 2]: m (base 2), l, o
+    float* part;             // [row][head][nsplit][HD]: the splits' weighted V sums
+    float2* part_ml;         // [row][head][nsplit]: their maximum (base 2) and weight sum
     float* out;
     uint8_t* outq8;
 };

@@ -19,6 +19,7 @@ const char* pages_fault(const axf_kv_pages* kv) {
         return "bad pool shape";
     if (kv->page_rows <= 0 || kv->page_rows > 1024 || (kv->page_rows & (kv->page_rows - 1)))
         return "page_rows must be a power of two up to 1024";
+    if ((long)kv->n_pages * kv->page_rows > 0x7fffffffL) return "more than 2^31 rows a layer";
     if (!aligned(kv->k, 16) || !aligned(kv->v, 16)) return "pages must be 16-byte aligned";
     return nullptr;
 }
@@ -157,6 +158,7 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
                 "n_heads must be a multiple of n_kv_heads up to 1024");
     AXF_REQUIRE(max_tok >= 0 && max_tok <= 64, "at most 64 tokens a sequence");
     AXF_REQUIRE(n_seq >= 0 && n_seq <= 65536 && max_len >= 0, "bad sizes");
+    AXF_REQUIRE((long)n_seq * max_tok * n_heads <= (1L << 26), "too many query rows");
     if (n_seq == 0 || max_tok == 0) return AXF_OK;
     AXF_REQUIRE(out && q && table && len, "null pointer");
     AXF_REQUIRE(!pos || (cos_t && sin_t && n_pos > 0), "pos needs the RoPE tables");
@@ -195,6 +197,8 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
         int rc = ctx_scratch(ctx, bytes, &scratch);
         if (rc) return rc;
         a.part = static_cast<float*>(scratch);
+        a.part_ml = reinterpret_cast<float2*>(
+            a.part + (size_t)n_seq * max_tok * n_heads * a.nsplit * kv->head_dim);
     }
     AXF_HIP(launch_attn_paged(a, kv->type, kv->head_dim, ctx->stream));
     return AXF_OK;

@@ -224,9 +224,10 @@ __device__ __forceinline__ uint64_t seen_mask(const PagedArgs& a, long row, int 
 }
 
 // One query row in plain fp32, a wave over the head's elements: the steps of 32 keys
-// step0, step0 + stride, ... of the span.  o: elements lane + 64 e.
+// step0, step0 + stride, ... of the span.  o: elements lane + 64 e.  (Arguments by
+// value: a reference would keep the kernels' own copies in memory.)
 template <int HD, class T>
-__device__ __noinline__ void row_careful(const PagedArgs& a, const Span& sp, int rho, int kvh, int step0,
+__device__ __noinline__ void row_careful(PagedArgs a, Span sp, int rho, int kvh, int step0,
                                          int stride, float& m, float& l, float* o) {
     constexpr int E = HD / 64;
     const int lane = threadIdx.x & 63, G = a.n_heads / a.n_kv_heads;
@@ -385,23 +386,19 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
     const T* kb = static_cast<const T*>(a.k) + kvh * HD + 8 * g;
     const T* vb = static_cast<const T*>(a.v) + kvh * HD + n * ND;
 
-    uint4 qf[NC][QP];
-    float scale;
-    load_q<HD, T>(a, sp, rho, kvh, live, qf, scale);
-    const uint64_t mask = live ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
-    f32x4 o[ND][SUMS];
-#pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < SUMS; e++) o[d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
-    // pool row of the lane's K key of each tile, -1: none
-    auto rows_of = [&](int jb, int (&r)[2]) {
+    // table entries of the lane's K key of each tile, kept as they are until their rows
+    // are asked for (arithmetic on them would wait for every load before theirs), and
+    // those rows, -1: none
+    auto pages_of = [&](int jb, int (&pg)[2]) {
 #pragma unroll
         for (int t = 0; t < 2; t++)
-            r[t] = (int)kv_row(min(jb + 16 * t + n, sp.j1 - 1), sp.table, a.table_ld, a.n_pages,
-                               a.page_shift);
+            pg[t] = kv_page(min(jb + 16 * t + n, sp.j1 - 1), sp.table, a.table_ld, a.page_shift);
+    };
+    auto rows_of = [&](int jb, const int (&pg)[2], int (&r)[2]) {
+#pragma unroll
+        for (int t = 0; t < 2; t++)
+            r[t] = (int)kv_row_of(min(jb + 16 * t + n, sp.j1 - 1), pg[t], a.table_ld, a.n_pages,
+                                  a.page_shift);
     };
     T kr[2][NC][8], vr[2][4][ND];
     auto load_k = [&](const int (&r)[2]) {
@@ -425,15 +422,26 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
             }
     };
     const int first = sp.j0 + wave * kStep, hop = kFewWaves * kStep;
-    int r[2], rn[2];
+    int r[2], rn[2], pg[2];
     if (first < sp.j1) {
-        rows_of(first, r);
+        pages_of(first, pg);
+        rows_of(first, pg, r);
         load_k(r);
         load_v(r);
+        pages_of(first + hop, pg);
     }
+    uint4 qf[NC][QP];
+    float scale;
+    load_q<HD, T>(a, sp, rho, kvh, live, qf, scale);
+    const uint64_t mask = live ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
+    f32x4 o[ND][SUMS];
+#pragma unroll
+    for (int d = 0; d < ND; d++)
+#pragma unroll
+        for (int e = 0; e < SUMS; e++) o[d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
     for (int jb = first; jb < sp.j1; jb += hop) {
         const bool more = jb + hop < sp.j1;
-        if (more) rows_of(jb + hop, rn);
         f32x4 st[2][SUMS];
 #pragma unroll
         for (int t = 0; t < 2; t++) {
@@ -458,7 +466,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
             for (int e = 0; e < 8; e++)
                 bad |= (uint32_t)(__shfl(r[e >> 2], 4 * g + (e & 3), 64) < 0) << e;
         }
-        if (more) load_k(rn);
+        if (more) {
+            rows_of(jb + hop, pg, rn);
+            load_k(rn);
+        }
         float keep;
         uint4 pf[QP];
         weights<T>(st, scale, hole || jb + kStep > min(sp.held, sp.j1), mask, jb, sp, bad, m, l, keep, pf);
@@ -484,6 +495,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
             load_v(rn);
             r[0] = rn[0];
             r[1] = rn[1];
+            pages_of(jb + 2 * hop, pg);
         }
     }
     // the wave's sums, element (4 g + e) * ND + d of row n
@@ -529,11 +541,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
     const int ro = tile * 16 + t;
     const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
     const bool whole = a.nsplit == 1 && !a.outq8;
-    float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * (HD + 2);
-    if (!whole && u == 0) {
-        dst[0] = top;
-        dst[1] = sum;
-    }
+    float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
+    if (!whole && u == 0) a.part_ml[orow * a.nsplit + split] = make_float2(top, sum);
     const float by = !whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
     for (int d = 4 * u; d < HD; d += 64) {
         float y[4] = {0.f, 0.f, 0.f, 0.f};
@@ -544,58 +553,286 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
             for (int e = 0; e < 4; e++) y[e] = fmaf(os[w][t][d + e], f[w], y[e]);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) dst[(whole ? 0 : 2) + d + e] = y[e] * by;
+        for (int e = 0; e < 4; e++) dst[d + e] = y[e] * by;
+    }
+}
+// ---- more rows: the workgroup's four waves share each step's K and V through LDS,
+// split into operands once (by the thread that loaded them) and laid out as the
+// operands' fragments (64 lanes x 16 bytes), so every LDS access is 1 KiB in a row.
+// Wave w has the 16-row tiles w, w + 4, ... of the workgroup's 64 MW rows; with MW = 2
+// a fragment read from LDS feeds two tiles' products.  The next step's values are in
+// flight while this one is multiplied.
+template <int HD, class T, int MW>
+__global__ __launch_bounds__(256, 2) void k_attn_paged_many(PagedArgs a, int tiles) {
+    constexpr int NC = HD / 32, ND = HD / 16, DV = HD / 64, KP = Parts<T>::KP, QP = Parts<T>::QP,
+                  SUMS = Parts<T>::SUMS;
+    __shared__ uint4 kl[2 * NC * KP * 64];
+    __shared__ uint4 vl[ND * KP * 64];
+    __shared__ uint32_t holes;  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
+    const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
+    const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
+    const int per = (a.n_kv_heads * a.nsplit + 7) & ~7;  // XCDs as in k_attn_paged_few
+    const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
+    const int tile = rest % tiles, cc = (rest / tiles) * 8 + xcd;
+    const int x = cc % per;
+    if (x >= a.n_kv_heads * a.nsplit) return;
+    const int kvh = x / a.nsplit, split = x % a.nsplit;
+    Span sp;
+    sp.s = cc / per;
+    const SeqLen len = seq_len(a.len, a.n_tok, a.max_tok, sp.s, a.table_ld, a.page_shift);
+    sp.held = len.held;
+    sp.tok = len.tok;
+    sp.table = a.table + (long)sp.s * a.table_ld;
+    const int total = sp.held + sp.tok, rows = sp.tok * G, row0 = tile * 64 * MW;
+    if (row0 >= rows) return;
+    sp.j0 = split * a.split_rows;
+    sp.j1 = split + 1 == a.nsplit ? total : min(total, sp.j0 + a.split_rows);
+    if (sp.j0 >= sp.j1 && split > 0) return;
+    const long ld = (long)a.n_kv_heads * HD;
+
+    // this thread's part of a step: K: key t & 15 of a tile, 8 elements; V: the 8 keys of
+    // group `wave`, DV elements
+    T kr[DV][8], vr[8][DV];
+    int pg[2];  // table entries of keys t & 15 of both tiles (as in k_attn_paged_few)
+    auto pages_of = [&](int jb) {
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++)
+            pg[tt] = kv_page(min(jb + 16 * tt + n, sp.j1 - 1), sp.table, a.table_ld, a.page_shift);
+    };
+    uint32_t bad = 0, bad_next = 0;
+    auto fetch = [&](int jb) {
+        int krow[2], vrow[8];
+#pragma unroll
+        for (int tt = 0; tt < 2; tt++)
+            krow[tt] = (int)kv_row_of(min(jb + 16 * tt + n, sp.j1 - 1), pg[tt], a.table_ld, a.n_pages,
+                                      a.page_shift);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            vrow[e] = __builtin_amdgcn_readlane(krow[e >> 2], 4 * wave + (e & 3));
+        const T* kb = static_cast<const T*>(a.k) + kvh * HD;
+        const T* vb = static_cast<const T*>(a.v) + kvh * HD + lane * DV;
+#pragma unroll
+        for (int p = 0; p < DV; p++) {
+            const int u = (t >> 4) + 16 * p, tt = u / (HD / 8), j = u % (HD / 8);
+            const int row = HD >= 128 ? krow[p / (HD / 128 ? HD / 128 : 1)] : (tt ? krow[1] : krow[0]);
+            __builtin_memcpy(kr[p], __builtin_assume_aligned(kb + (long)max(row, 0) * ld + 8 * j, 16),
+                             8 * sizeof(T));
+        }
+        bad_next = 0;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            bad_next |= (uint32_t)(vrow[e] < 0) << e;
+            __builtin_memcpy(vr[e],
+                             __builtin_assume_aligned(vb + (long)max(vrow[e], 0) * ld, DV * sizeof(T)),
+                             DV * sizeof(T));
+        }
+    };
+    auto put = [&] {  // split what was fetched into LDS
+#pragma unroll
+        for (int p = 0; p < DV; p++) {
+            const int u = (t >> 4) + 16 * p, tt = u / (HD / 8), j = u % (HD / 8);
+            uint4 f[KP];
+            if constexpr (KP == 1)
+                __builtin_memcpy(&f[0], kr[p], 16);
+            else
+                Parts<T>::split_kv(kr[p], f);
+#pragma unroll
+            for (int q = 0; q < KP; q++)
+                kl[((tt * NC + j / 4) * KP + q) * 64 + (j & 3) * 16 + (t & 15)] = f[q];
+        }
+#pragma unroll
+        for (int e = 0; e < DV; e++) {
+            const int d = lane * DV + e;
+            T w[8];
+#pragma unroll
+            for (int r = 0; r < 8; r++) w[r] = vr[r][e];
+            uint4 f[KP];
+            if constexpr (KP == 1)
+                __builtin_memcpy(&f[0], w, 16);
+            else
+                Parts<T>::split_kv(w, f);
+#pragma unroll
+            for (int q = 0; q < KP; q++) vl[((d >> 4) * KP + q) * 64 + wave * 16 + (d & 15)] = f[q];
+        }
+        if (lane == 0) reinterpret_cast<uint8_t*>(&holes)[wave] = (uint8_t)bad_next;
+    };
+
+    pages_of(sp.j0);
+    fetch(sp.j0);
+    pages_of(sp.j0 + kStep);
+
+    uint4 qf[MW][NC][QP];
+    float scale[MW], m[MW], l[MW];
+    uint64_t mask[MW];
+    bool act[MW], live[MW];
+    f32x4 o[MW][ND][SUMS];
+#pragma unroll
+    for (int w = 0; w < MW; w++) {
+        const int rho = row0 + (wave + 4 * w) * 16 + n;
+        act[w] = row0 + (wave + 4 * w) * 16 < rows;
+        live[w] = rho < rows;
+        load_q<HD, T>(a, sp, rho, kvh, live[w], qf[w], scale[w]);
+        mask[w] = live[w] ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
+        m[w] = -INFINITY;
+        l[w] = 0.f;
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < SUMS; e++) o[w][d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int jb = sp.j0; jb < sp.j1; jb += kStep) {
+        put();
+        if (jb + kStep < sp.j1) {
+            fetch(jb + kStep);
+            pages_of(jb + 2 * kStep);
+        }
+        __syncthreads();
+        if (act[0]) {
+            f32x4 st[MW][2][SUMS];
+#pragma unroll
+            for (int w = 0; w < MW; w++)
+#pragma unroll
+                for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                    for (int e = 0; e < SUMS; e++) st[w][tt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int tt = 0; tt < 2; tt++)
+#pragma unroll
+                for (int c = 0; c < NC; c++) {
+                    uint4 f[KP];
+#pragma unroll
+                    for (int q = 0; q < KP; q++) f[q] = kl[((tt * NC + c) * KP + q) * 64 + lane];
+#pragma unroll
+                    for (int w = 0; w < MW; w++)
+                        if (w == 0 || act[w]) Parts<T>::product(f, qf[w][c], st[w][tt]);
+                }
+            const uint32_t hole = holes;
+            bad = (hole >> (8 * g)) & 255;
+            uint4 pf[MW][QP];
+#pragma unroll
+            for (int w = 0; w < MW; w++) {
+                if (w > 0 && !act[w]) continue;
+                float keep;
+                weights<T>(st[w], scale[w], hole || jb + kStep > min(sp.held, sp.j1), mask[w], jb, sp,
+                           bad, m[w], l[w], keep, pf[w]);
+#pragma unroll
+                for (int d = 0; d < ND; d++)
+#pragma unroll
+                    for (int e = 0; e < SUMS; e++) o[w][d][e] *= keep;
+            }
+#pragma unroll
+            for (int d = 0; d < ND; d++) {
+                uint4 f[KP];
+#pragma unroll
+                for (int q = 0; q < KP; q++) f[q] = vl[(d * KP + q) * 64 + lane];
+#pragma unroll
+                for (int w = 0; w < MW; w++)
+                    if (w == 0 || act[w]) Parts<T>::product(f, pf[w], o[w][d]);
+            }
+        }
+        __syncthreads();
+    }
+    const bool whole = a.nsplit == 1 && !a.outq8;
+#pragma unroll
+    for (int w = 0; w < MW; w++) {
+        if (!act[w]) continue;
+        l[w] = rows_sum(l[w]);
+        float check = l[w];
+#pragma unroll
+        for (int d = 0; d < ND; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) check = fmaf(Parts<T>::total(o[w][d], e), 0.f, check);
+        const int tile0 = row0 + (wave + 4 * w) * 16;
+        if (__any(live[w] && !(fabsf(check) < INFINITY))) {
+            for (int i = 0; i < 16 && tile0 + i < rows; i++) {
+                float mc, lc, oc[HD / 64];
+                row_careful<HD, T>(a, sp, tile0 + i, kvh, 0, 1, mc, lc, oc);
+                const int ro = tile0 + i;
+                const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
+                float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
+                if (!whole && lane == 0) a.part_ml[orow * a.nsplit + split] = make_float2(mc, lc);
+                for (int e = 0; e < HD / 64; e++)
+                    dst[lane + 64 * e] = !whole ? oc[e] : (lc == 0.f ? 0.f : oc[e] / lc);
+            }
+            continue;
+        }
+        if (!live[w]) continue;
+        const int ro = tile0 + n;
+        const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
+        float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
+        if (!whole && g == 0) a.part_ml[orow * a.nsplit + split] = make_float2(m[w], l[w]);
+        const float by = !whole ? 1.f : (l[w] == 0.f ? 0.f : 1.f / l[w]);
+#pragma unroll
+        for (int d = 0; d < ND; d++) {
+            f32x4_a4 y;
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = Parts<T>::total(o[w][d], e) * by;
+            *reinterpret_cast<f32x4_a4*>(dst + 16 * d + 4 * g) = y;
+        }
     }
 }
 
-// Partial result of a split: m, l (sum of 2^(t - m)) and o (the weighted V sum).
 // One wave a query row and head: the splits' sums brought to one base and added
-// in their order, divided by the weights' sum.
+// in their order, divided by the weights' sum.  Lane j has split j's m and l (at most
+// 64 splits), so one load's latency covers them all.
 template <int HD>
 __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a) {
-    constexpr int E = HD / 64;
+    constexpr int E = HD / 64, U = 8;
     const int lane = threadIdx.x & 63;
     const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (w >= (long)a.n_seq * a.max_tok * a.n_heads) return;
-    const int h = (int)(w % a.n_heads);
     const long row = w / a.n_heads;
     const int s = (int)(row / a.max_tok);
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
     if ((int)(row % a.max_tok) >= n.tok) return;
-    const int used = min(a.nsplit, (n.held + n.tok + a.split_rows - 1) / a.split_rows);
-    const float* p = a.part + w * a.nsplit * (HD + 2);
-    float top = -INFINITY;
-    for (int j = 0; j < used; j++) top = fmaxf(top, p[(long)j * (HD + 2)]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float l = 0.f, o[E];
+    const int used = __builtin_amdgcn_readfirstlane(
+        min(a.nsplit, (n.held + n.tok + a.split_rows - 1) / a.split_rows));
+    const float2 ml = lane < used ? a.part_ml[w * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
+    const float* p = a.part + w * a.nsplit * HD + lane * E;
+    const float top = wave_max(ml.x);
+    const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
+    const float l = wave_sum(ml.y * f);
+    float o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) o[e] = 0.f;
-    for (int j = 0; j < used; j++) {
-        const float* pj = p + (long)j * (HD + 2);
-        if (pj[1] == 0.f) continue;  // no weight there, whatever it holds
-        const float f = exp2f(pj[0] - base);
-        l = fmaf(pj[1], f, l);
+    for (int j0 = 0; j0 < used; j0 += U) {
+        float v[U][E];
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = fmaf(pj[2 + lane + 64 * e], f, o[e]);
+        for (int j = 0; j < U; j++)
+#pragma unroll
+            for (int e = 0; e < E; e++) v[j][e] = p[(long)min(j0 + j, used - 1) * HD + e];
+#pragma unroll
+        for (int j = 0; j < U; j++) {
+            const float fj = j0 + j < used ? __uint_as_float(__builtin_amdgcn_readlane(
+                                                 __float_as_uint(f), (j0 + j) & 63))
+                                           : 0.f;
+            if (fj == 0.f) continue;
+#pragma unroll
+            for (int e = 0; e < E; e++) o[e] = fmaf(v[j][e], fj, o[e]);
+        }
     }
-    float* dst = a.out + row * a.n_heads * HD + h * HD;
+    float* dst = a.out + w * HD + lane * E;
+    const float by = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        const float y = l == 0.f ? 0.f : o[e] / l;
-        dst[lane + 64 * e] = y;
-        if (a.outq8) {
-            // lane & 31 of each half wave holds one block's values
-            float amax = fabsf(y);
+        o[e] *= by;
+        dst[e] = o[e];
+    }
+    if (a.outq8) {
+        // a block's 32 values are in 32 / E neighbouring lanes
+        float amax = 0.f;
 #pragma unroll
-            for (int off = 16; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
-            const float id = amax > 0.f ? 127.f / amax : 0.f;
-            const float r = fminf(fmaxf(rintf(y * id), -128.f), 127.f);
-            const int b = __builtin_isinf(id) ? -128 : (int)r;
-            uint8_t* blk = a.outq8 +
-                           ((row * a.n_heads + h) * (HD / 32) + e * 2 + (lane >> 5)) * Q8_0_BYTES;
-            blk[4 + (lane & 31)] = (uint8_t)b;
-            if ((lane & 31) == 0) *reinterpret_cast<float*>(blk) = amax / 127.f;
+        for (int e = 0; e < E; e++) amax = fmaxf(amax, fabsf(o[e]));
+#pragma unroll
+        for (int off = 16 / E; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
+        const float id = amax > 0.f ? 127.f / amax : 0.f;
+        uint8_t* blk = a.outq8 + (w * (HD / 32) + lane * E / 32) * Q8_0_BYTES;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const float r = fminf(fmaxf(rintf(o[e] * id), -128.f), 127.f);
+            blk[4 + (lane * E + e) % 32] = (uint8_t)(__builtin_isinf(id) ? -128 : (int)r);
         }
+        if ((lane * E) % 32 == 0) *reinterpret_cast<float*>(blk) = amax / 127.f;
     }
 }
 
@@ -879,12 +1116,25 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
     len_out[s] = kv_len(len[s], table_ld, page_shift) + n;
 }
 
+// Query rows of a KV head that a workgroup takes (attn_paged_plan has the rule).
+int tile_rows(int rows, int head_dim) {
+    if (rows <= 16) return 16;
+    return rows <= 64 || head_dim == 256 ? 64 : 128;
+}
+
 template <int HD, class T>
 hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
-    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads);
-    const int tiles = (rows + 15) / 16;
+    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, HD);
+    const int tiles = (rows + tr - 1) / tr;
     const long per = (a.n_kv_heads * a.nsplit + 7) & ~7;
-    k_attn_paged_few<HD, T><<<(unsigned)(per * a.n_seq * tiles), 64 * kFewWaves, 0, st>>>(a, tiles);
+    const unsigned wgs = (unsigned)(per * a.n_seq * tiles);
+    if (tr == 16) {
+        k_attn_paged_few<HD, T><<<wgs, 64 * kFewWaves, 0, st>>>(a, tiles);
+    } else if (tr == 64) {
+        k_attn_paged_many<HD, T, 1><<<wgs, 256, 0, st>>>(a, tiles);
+    } else {
+        if constexpr (HD < 256) k_attn_paged_many<HD, T, 2><<<wgs, 256, 0, st>>>(a, tiles);
+    }
     if (a.nsplit > 1 || a.outq8) {
         const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
         k_attn_paged_join<HD><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
@@ -903,14 +1153,14 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 
 void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     (void)kv_type;
-    (void)head_dim;
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
-    const long tiles = (a.max_tok * (a.n_heads / a.n_kv_heads) + 15) / 16;
-    const long parts = (long)a.n_seq * a.n_kv_heads * tiles;
-    const long unit = kStep * kFewWaves;
-    long split = longest * parts / 1024;
+    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, head_dim);
+    const long parts = (long)a.n_seq * a.n_kv_heads * ((rows + tr - 1) / tr);
+    const long unit = tr == 16 ? kStep * kFewWaves : 2 * kStep;
+    long split = longest * parts / (tr == 16 ? 1024 : 768);
     split = split < unit ? unit : (split + unit - 1) / unit * unit;
+    while ((longest + split - 1) / split > 64) split += unit;  // the join's lanes
     a.split_rows = (int)split;
     a.nsplit = (int)((longest + split - 1) / split);
 }

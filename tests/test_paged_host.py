@@ -58,7 +58,8 @@ def call_args(base, **kw):
                                  dict(n_pages=0), dict(n_pages=-1), dict(page_rows=0),
                                  dict(page_rows=24), dict(page_rows=2048), dict(n_kv_heads=0),
                                  dict(n_kv_heads=257), dict(head_dim=96), dict(k=D + 8),
-                                 dict(v=D + 4), dict(n_layers=20000)])
+                                 dict(v=D + 4), dict(n_layers=20000),
+                                 dict(n_pages=1 << 28, page_rows=16)])
 @pytest.mark.parametrize("name", [n for n in CALLS if "kv" in CALLS[n]])
 def test_bad_pools_are_refused(name, bad):
     refused(name, call_args(CALLS[name], kv=C.byref(pool(**bad))))
@@ -79,7 +80,8 @@ def test_bad_pools_are_refused(name, bad):
         "axf_hip_attn_paged": [dict(out=None), dict(q=None), dict(q_ld=511), dict(layer=2),
                                dict(table=None), dict(table_ld=0), dict(len=None), dict(cos=None),
                                dict(n_pos=0), dict(n_seq=-1), dict(max_tok=65), dict(max_tok=-1),
-                               dict(max_len=-1), dict(n_heads=0), dict(n_heads=3),
+                               dict(max_len=-1), dict(n_seq=65536, max_tok=64, n_heads=32, q_ld=1 << 14),
+                               dict(n_heads=0), dict(n_heads=3),
                                dict(n_heads=2048), dict(mask=D + 4), dict(out=D + 2),
                                dict(outq8=D + 2), dict(q=D + 1)],
         "axf_hip_kv_compact": [dict(len_out=None), dict(table=None), dict(len=None),
