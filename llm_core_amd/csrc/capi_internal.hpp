@@ -337,15 +337,18 @@ struct PagedArgs {
     const float *cos_t, *sin_t;
     int n_pos, n_seq, max_tok, n_heads, n_kv_heads;
     int n_pages, page_shift;
-    int nsplit, split_rows;  // split j: positions [j * split_rows, ...), the last one to the end
-    float* part;             // [row][head][nsplit][HD]: the splits' weighted V sums
-    float2* part_ml;         // [row][head][nsplit]: their maximum (base 2) and weight sum
     float* out;
     uint8_t* outq8;
+    int shares;       // workgroups that the keys are dealt out to (attn_paged_plan)
+    // set by the launcher, in its scratch
+    float* part;      // [share][2][tile rows][HD]: unfinished weighted V sums
+    float2* part_ml;  // [share][2][tile rows]: their maximum (base 2) and weight sum
+    long* plan;       // units before each sequence
 };
-void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len);
+void attn_paged_plan(PagedArgs& a, int head_dim, int max_len);
 size_t attn_paged_scratch(const PagedArgs& a, int head_dim);
-hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, hipStream_t st);
+hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, void* scratch,
+                             hipStream_t st);
 struct KvStoreArgs {
     void *k, *v;  // layer's first page
     const int* table;

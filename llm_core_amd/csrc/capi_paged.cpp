@@ -191,16 +191,11 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
     a.page_shift = page_shift(kv);
     a.out = out;
     a.outq8 = static_cast<uint8_t*>(outq8);
-    attn_paged_plan(a, kv->type, kv->head_dim, max_len);
-    if (const size_t bytes = attn_paged_scratch(a, kv->head_dim)) {
-        void* scratch = nullptr;
-        int rc = ctx_scratch(ctx, bytes, &scratch);
-        if (rc) return rc;
-        a.part = static_cast<float*>(scratch);
-        a.part_ml = reinterpret_cast<float2*>(
-            a.part + (size_t)n_seq * max_tok * n_heads * a.nsplit * kv->head_dim);
-    }
-    AXF_HIP(launch_attn_paged(a, kv->type, kv->head_dim, ctx->stream));
+    attn_paged_plan(a, kv->head_dim, max_len);
+    void* scratch = nullptr;
+    int rc = ctx_scratch(ctx, attn_paged_scratch(a, kv->head_dim), &scratch);
+    if (rc) return rc;
+    AXF_HIP(launch_attn_paged(a, kv->type, kv->head_dim, scratch, ctx->stream));
     return AXF_OK;
 }
 

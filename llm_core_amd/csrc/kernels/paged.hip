@@ -5,6 +5,8 @@
 #include "common.hpp"
 #include "paged_index.hpp"
 
+#include <type_traits>
+
 namespace axf {
 
 namespace {
@@ -59,11 +61,13 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
 //   F32 pages: x = h + m + l, three bf16 cut off one after the other (exact: 8 bits
 //   each, the whole range of fp32, no scales), and the six products that reach 2^-24
 //   of the largest: hh, hm, mh, mm, hl, lh; 6/16 of the fp32 matrix rate's time.
-//   F16 pages: K and V are fp16 as they are; q (scaled by a power of two a row) and p
-//   are h + 2^-12 l, two fp16 parts with a sum of their own each, 22 bits: two
-//   products and no work on K or V.
-// Infinities and NaN do not split; a wave whose sums end up not finite does its rows
-// again in plain fp32 (row_careful), where each masked place is left out.
+//   F16 pages: K and V are fp16 as they are; q (scaled by a power of two a row) is
+//   h + 2^-12 l, two fp16 parts with a sum of their own each, 22 bits of every element;
+//   p (times 2^15) is h + l with one sum, 22 bits down to p = 2^-16 and 2^-39 below
+//   (a second sum would cost O's registers again): two products, no work on K or V.
+// Infinities and NaN do not split, and 0 times one of them in a masked place is NaN: a
+// row whose result is not finite is done again in plain fp32 (row_careful, by the
+// joining kernel), where masked places are left out.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -87,13 +91,15 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 }
 
 // How values of a page type become 16-bit operands.  KP / QP: parts of K and V, of q
-// and p; SUMS: accumulators a product needs.
+// and p; SUMS: accumulators of q's product; kUp: what O is too large by.
 template <class T>
 struct Parts;
 
 template <>
 struct Parts<float> {
     static constexpr int KP = 3, QP = 3, SUMS = 1;
+    static constexpr float kUp = 1.f;
+    static constexpr bool kScaleQ = false;
     static __device__ __forceinline__ void split(const float (&x)[8], uint4 (&f)[3]) {
         uint32_t w[3][4];
 #pragma unroll
@@ -109,53 +115,87 @@ struct Parts<float> {
         for (int p = 0; p < 3; p++) f[p] = make_uint4(w[p][0], w[p][1], w[p][2], w[p][3]);
     }
     static __device__ __forceinline__ void split_q(const float (&x)[8], uint4 (&f)[3]) { split(x, f); }
+    static __device__ __forceinline__ void split_p(const float (&x)[8], uint4 (&f)[3]) { split(x, f); }
     static __device__ __forceinline__ void split_kv(const float (&x)[8], uint4 (&f)[3]) { split(x, f); }
     static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
                                                        __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
     }
-    // the smallest products first
-    static __device__ __forceinline__ void product(const uint4 (&a)[3], const uint4 (&b)[3],
-                                                   f32x4 (&c)[1]) {
-        c[0] = mul(a[2], b[0], c[0]);
-        c[0] = mul(a[0], b[2], c[0]);
-        c[0] = mul(a[1], b[1], c[0]);
-        c[0] = mul(a[1], b[0], c[0]);
-        c[0] = mul(a[0], b[1], c[0]);
-        c[0] = mul(a[0], b[0], c[0]);
+    // c[i][j] += a[i] b[j], NA x NB products side by side (the six sums of one wait for
+    // each other), the smallest first
+    template <int NA, int NB>
+    static __device__ __forceinline__ void product(const uint4 (&a)[NA][3], const uint4* const (&b)[NB],
+                                                   f32x4* const (&c)[NA][NB]) {
+        constexpr int A[6] = {2, 0, 1, 1, 0, 0}, B[6] = {0, 2, 1, 0, 1, 0};
+#pragma unroll
+        for (int p = 0; p < 6; p++)
+#pragma unroll
+            for (int i = 0; i < NA; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) *c[i][j] = mul(a[i][A[p]], b[j][B[p]], *c[i][j]);
+    }
+    // the same for scores, whose sums are SUMS apart
+    template <int NA, int NB>
+    static __device__ __forceinline__ void scores(const uint4 (&a)[NA][3], const uint4* const (&b)[NB],
+                                                  f32x4* const (&c)[NA][NB]) {
+        product<NA, NB>(a, b, c);
     }
     static __device__ __forceinline__ float total(const f32x4 (&c)[1], int r) { return c[0][r]; }
-    static constexpr bool kScaleQ = false;
 };
 
 template <>
 struct Parts<_Float16> {
     static constexpr int KP = 1, QP = 2, SUMS = 2;
-    static __device__ __forceinline__ void split_q(const float (&x)[8], uint4 (&f)[2]) {
+    static constexpr float kUp = 32768.f;
+    static constexpr bool kScaleQ = true;
+    static __device__ __forceinline__ void split(const float (&x)[8], float low, uint4 (&f)[2]) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float a = x[2 * e], b = x[2 * e + 1];
             const float a0 = (float)(_Float16)a, b0 = (float)(_Float16)b;
             h[e] = pack_f16(a, b);
-            l[e] = pack_f16((a - a0) * 4096.f, (b - b0) * 4096.f);
+            l[e] = pack_f16((a - a0) * low, (b - b0) * low);
         }
         f[0] = make_uint4(h[0], h[1], h[2], h[3]);
         f[1] = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+    static __device__ __forceinline__ void split_q(const float (&x)[8], uint4 (&f)[2]) {
+        split(x, 4096.f, f);
+    }
+    static __device__ __forceinline__ void split_p(const float (&x)[8], uint4 (&f)[2]) {
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = x[e] * kUp;
+        split(y, 1.f, f);
     }
     static __device__ __forceinline__ f32x4 mul(const uint4& a, const uint4& b, f32x4 c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
                                                       __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
     }
-    static __device__ __forceinline__ void product(const uint4 (&a)[1], const uint4 (&b)[2],
-                                                   f32x4 (&c)[2]) {
-        c[0] = mul(a[0], b[0], c[0]);
-        c[1] = mul(a[0], b[1], c[1]);
+    template <int NA, int NB>
+    static __device__ __forceinline__ void product(const uint4 (&a)[NA][1], const uint4* const (&b)[NB],
+                                                   f32x4* const (&c)[NA][NB]) {
+#pragma unroll
+        for (int p = 1; p >= 0; p--)
+#pragma unroll
+            for (int i = 0; i < NA; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) *c[i][j] = mul(a[i][0], b[j][p], *c[i][j]);
+    }
+    template <int NA, int NB>
+    static __device__ __forceinline__ void scores(const uint4 (&a)[NA][1], const uint4* const (&b)[NB],
+                                                  f32x4* const (&c)[NA][NB]) {
+#pragma unroll
+        for (int p = 0; p < 2; p++)
+#pragma unroll
+            for (int i = 0; i < NA; i++)
+#pragma unroll
+                for (int j = 0; j < NB; j++) c[i][j][p] = mul(a[i][0], b[j][p], c[i][j][p]);
     }
     static __device__ __forceinline__ float total(const f32x4 (&c)[2], int r) {
         return fmaf(c[1][r], 1.f / 4096.f, c[0][r]);
     }
-    static constexpr bool kScaleQ = true;
 };
 
 // Reductions over the four 16-lane rows of a wave (lanes n, n + 16, n + 32, n + 48),
@@ -213,69 +253,160 @@ __device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, i
     }
 }
 
-// What a wave needs to know of its sequence and split.
+// How the work is split.  A part is one sequence's, KV head's and row tile's walk over
+// its keys, in units of `unit` keys; all parts' units in a row are dealt out evenly to
+// the grid's workgroups, which are as many as run at once: every workgroup has the same
+// number of units, however ragged the lengths, and a part that lies in one share is
+// finished there.  A share holds at most two unfinished ends (its first part's and its
+// last's); they go to the workgroup's two slots of partial sums, which
+// k_attn_paged_join adds.
+constexpr int kPlanSeqs = 256;  // sequences a launch
+
+struct SeqWork {
+    int rows, tiles;
+    long units;  // of one part
+};
+__device__ __forceinline__ SeqWork seq_work(const SeqLen& n, int G, int tile_rows, int unit) {
+    SeqWork w;
+    w.rows = n.tok * G;
+    w.tiles = (w.rows + tile_rows - 1) / tile_rows;
+    w.units = w.tiles ? ((long)n.held + n.tok + unit - 1) / unit : 0;
+    return w;
+}
+
+// cum[s]: units before sequence s (cum[n_seq]: all); the first 256 threads.
+__device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, int unit, long* cum,
+                                          long* part) {
+    const int t = threadIdx.x, lane = t & 63;
+    long w = 0;
+    if (t < a.n_seq) {
+        const SeqWork k = seq_work(seq_len(a.len, a.n_tok, a.max_tok, t, a.table_ld, a.page_shift),
+                                   a.n_heads / a.n_kv_heads, tile_rows, unit);
+        w = k.units * k.tiles * a.n_kv_heads;
+    }
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) {
+        const long y = __shfl_up(w, off, 64);
+        if (lane >= off) w += y;
+    }
+    if (lane == 63 && t < kPlanSeqs) part[t >> 6] = w;
+    __syncthreads();
+    if (t < kPlanSeqs) {
+        for (int i = 0; i < (t >> 6); i++) w += part[i];
+        cum[t + 1] = w;
+    }
+    if (t == 0) cum[0] = 0;
+    __syncthreads();
+}
+
+// Shares that have units (none is empty before the last), the first unit of share w of
+// n, and the share that unit u is in.
+__device__ __forceinline__ int shares_used(const PagedArgs& a, long total) {
+    return (int)min((long)a.shares, total);
+}
+__device__ __forceinline__ long share_start(long total, int w, int n) { return total * w / n; }
+__device__ __forceinline__ int share_of(long total, long u, int n) {
+    return (int)(((u + 1) * n - 1) / total);
+}
+
+// One part's stretch of keys in a share.
 struct Span {
     int s, held, tok, j0, j1;
     const int* table;
+    int rows, kvh, tile;
+    int slot;  // of partial sums, -1: the whole part
 };
+
+// The stretch at unit lo of a share that ends at hi; moves lo behind it.
+__device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, int tile_rows, int unit,
+                                          int share, int& s, long& lo, long hi) {
+    while (lo >= cum[s + 1]) s++;
+    Span p;
+    p.s = __builtin_amdgcn_readfirstlane(s);
+    const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, p.s, a.table_ld, a.page_shift);
+    const SeqWork w = seq_work(n, a.n_heads / a.n_kv_heads, tile_rows, unit);
+    p.held = n.held;
+    p.tok = n.tok;
+    p.rows = w.rows;
+    p.table = a.table + (long)p.s * a.table_ld;
+    const long at = lo - cum[p.s], part = at / w.units, u0 = at - part * w.units;
+    const long u1 = min(w.units, u0 + hi - lo);
+    p.kvh = __builtin_amdgcn_readfirstlane((int)(part / w.tiles));
+    p.tile = __builtin_amdgcn_readfirstlane((int)(part % w.tiles));
+    p.j0 = __builtin_amdgcn_readfirstlane((int)(u0 * unit));
+    p.j1 = __builtin_amdgcn_readfirstlane((int)min(u1 * unit, (long)n.held + n.tok));
+    p.slot = u0 > 0 ? 2 * share : (u1 < w.units ? 2 * share + 1 : -1);
+    lo += u1 - u0;
+    return p;
+}
 
 __device__ __forceinline__ uint64_t seen_mask(const PagedArgs& a, long row, int i) {
     return a.mask ? a.mask[row] : ~0ull >> (63 - i);
 }
 
-// One query row in plain fp32, a wave over the head's elements: the steps of 32 keys
-// step0, step0 + stride, ... of the span.  o: elements lane + 64 e.  (Arguments by
-// value: a reference would keep the kernels' own copies in memory.)
+// One query row in plain fp32, a wave over the head's elements (o: elements
+// E lane ..), four keys at a time.
 template <int HD, class T>
-__device__ __noinline__ void row_careful(PagedArgs a, Span sp, int rho, int kvh, int step0,
-                                         int stride, float& m, float& l, float* o) {
-    constexpr int E = HD / 64;
-    const int lane = threadIdx.x & 63, G = a.n_heads / a.n_kv_heads;
-    const int i = rho / G, h = kvh * G + rho % G;
-    const long row = (long)sp.s * a.max_tok + i, ld = (long)a.n_kv_heads * HD;
+__device__ __forceinline__ void row_careful(const PagedArgs& a, int s, int i, int h, float (&y)[HD / 64]) {
+    constexpr int E = HD / 64, U = 4;
+    const int lane = threadIdx.x & 63, kvh = h / (a.n_heads / a.n_kv_heads);
+    const long row = (long)s * a.max_tok + i, ld = (long)a.n_kv_heads * HD;
+    const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
+    const int* table = a.table + (long)s * a.table_ld;
     const uint64_t mask = seen_mask(a, row, i);
-    const T* k = static_cast<const T*>(a.k) + kvh * HD;
-    const T* v = static_cast<const T*>(a.v) + kvh * HD;
+    const T* k = static_cast<const T*>(a.k) + kvh * HD + lane * E;
+    const T* v = static_cast<const T*>(a.v) + kvh * HD + lane * E;
     const float c = kLog2e / sqrtf((float)HD);
-    float q[E];
+    float q[E], o[E];
 #pragma unroll
     for (int e = 0; e < E; e++) {
-        q[e] = q_value<HD>(a, row, h, lane + 64 * e);
+        q[e] = q_value<HD>(a, row, h, lane * E + e);
         o[e] = 0.f;
     }
-    m = -INFINITY;
-    l = 0.f;
-    for (int b = sp.j0 + step0 * kStep; b < sp.j1; b += stride * kStep) {
-        for (int j = b; j < min(b + kStep, sp.j1); j++) {
-            if (j >= sp.held && !((mask >> (j - sp.held)) & 1)) continue;
-            const long r = kv_row(j, sp.table, a.table_ld, a.n_pages, a.page_shift);
-            if (r < 0) continue;
-            float d = 0.f;
+    float m = -INFINITY, l = 0.f;
+    const int total = n.held + n.tok;
+    for (int j0 = 0; j0 < total; j0 += U) {
+        float d[U], w[U][E];
 #pragma unroll
-            for (int e = 0; e < E; e++) d = fmaf(q[e], (float)k[r * ld + lane + 64 * e], d);
-            d = wave_sum(d) * c;
-            if (d == -INFINITY) continue;  // no weight, whatever the value
-            const float mn = fmaxf(m, d);
+        for (int u = 0; u < U; u++) {
+            const int j = min(j0 + u, total - 1);
+            const long r = kv_row(j, table, a.table_ld, a.n_pages, a.page_shift);
+            const bool see = j0 + u < total && r >= 0 &&
+                             (j < n.held || ((mask >> (j - n.held)) & 1));
+            float x = 0.f;
+#pragma unroll
+            for (int e = 0; e < E; e++) {
+                x = fmaf(q[e], (float)k[max(r, 0L) * ld + e], x);
+                w[u][e] = (float)v[max(r, 0L) * ld + e];
+            }
+            x = wave_sum(x) * c;
+            d[u] = see ? x : -INFINITY;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            if (d[u] == -INFINITY) continue;  // no weight, whatever the value
+            const float mn = fmaxf(m, d[u]);
             const float base = mn == -INFINITY ? 0.f : mn;
-            const float keep = exp2f(m - base), p = exp2f(d - base);
+            const float keep = exp2f(m - base), p = exp2f(d[u] - base);
             l = l * keep + p;
 #pragma unroll
-            for (int e = 0; e < E; e++)
-                o[e] = fmaf(p, (float)v[r * ld + lane + 64 * e], keep == 0.f ? 0.f : o[e] * keep);
+            for (int e = 0; e < E; e++) o[e] = fmaf(p, w[u][e], keep == 0.f ? 0.f : o[e] * keep);
             m = mn;
         }
     }
+#pragma unroll
+    for (int e = 0; e < E; e++) y[e] = l == 0.f ? 0.f : o[e] / l;
 }
 
 // q's fragments of one 16-row tile: lane's row, elements 32 c + 8 (lane >> 4) .. +7 of
 // each 32-element chunk.  scale: what scores are multiplied by (with F16 pages the
 // row was scaled to the top of fp16's range).
 template <int HD, class T>
-__device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, int kvh, bool live,
+__device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, bool live,
                                        uint4 (&qf)[HD / 32][Parts<T>::QP], float& scale) {
     constexpr int NC = HD / 32;
     const int g = (threadIdx.x & 63) >> 4, G = a.n_heads / a.n_kv_heads;
-    const int i = rho / G, h = kvh * G + rho % G;
+    const int i = rho / G, h = sp.kvh * G + rho % G;
     float x[NC][8];
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -286,7 +417,8 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int r
             for (int e = 0; e < 8; e++) x[c][e] = 0.f;
         }
     }
-    scale = kLog2e / sqrtf((float)HD);
+    constexpr float kRoot = HD == 64 ? 8.f : HD == 256 ? 16.f : 11.3137084989847603904f;
+    scale = kLog2e / kRoot;
     float up = 1.f;
     if (Parts<T>::kScaleQ) {
         float top = 0.f;
@@ -344,42 +476,50 @@ __device__ __forceinline__ void weights(const f32x4 (&st)[2][Parts<T>::SUMS], fl
     }
     l = fmaf(l, keep, sum);
     m = mn;
-    Parts<T>::split_q(p, pf);
+    Parts<T>::split_p(p, pf);
 }
 
 // ---- up to 16 query rows: a wave needs every K and V value once, so it loads them
 // from memory straight into the operands' layout (K: lane's key row, 8 elements a chunk;
 // V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
 // waves take every fourth step of the split and join at its end.
-constexpr int kFewWaves = 4;
+constexpr int kFewWaves = 4, kFewUnit = kFewWaves * kStep;
+
+// Shares that follow each other run on one XCD (workgroups go round the XCDs): their
+// parts' row tiles, or beams' shared pages, are in one L2.
+__device__ __forceinline__ int share_id() {
+    const int n = gridDim.x;  // a multiple of 8
+    return (blockIdx.x & 7) * (n >> 3) + (blockIdx.x >> 3);
+}
+
+// Row of out (of HD floats) that query row rho of a span is.
+__device__ __forceinline__ long out_row(const PagedArgs& a, const Span& sp, int rho) {
+    const int G = a.n_heads / a.n_kv_heads;
+    return ((long)sp.s * a.max_tok + rho / G) * a.n_heads + sp.kvh * G + rho % G;
+}
 
 template <int HD, class T>
-__global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, int tiles) {
+__global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) {
     constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
                   SUMS = Parts<T>::SUMS;
     __shared__ float os[kFewWaves][16][HD + 4];
     __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
+    __shared__ long cum[kPlanSeqs + 1], scan[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
-    // workgroups of one part of the cache (its row tiles; other sequences' same part,
-    // which may be the same pages) are 8 apart: one XCD's L2 serves them
-    const int per = (a.n_kv_heads * a.nsplit + 7) & ~7;
-    const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
-    const int tile = rest % tiles, c = (rest / tiles) * 8 + xcd;
-    const int x = c % per;
-    if (x >= a.n_kv_heads * a.nsplit) return;
-    const int kvh = x / a.nsplit, split = x % a.nsplit;
-    Span sp;
-    sp.s = c / per;
-    const SeqLen len = seq_len(a.len, a.n_tok, a.max_tok, sp.s, a.table_ld, a.page_shift);
-    sp.held = len.held;
-    sp.tok = len.tok;
-    sp.table = a.table + (long)sp.s * a.table_ld;
-    const int total = sp.held + sp.tok, rows = sp.tok * G;
-    if (tile * 16 >= rows) return;
-    sp.j0 = split * a.split_rows;
-    sp.j1 = split + 1 == a.nsplit ? total : min(total, sp.j0 + a.split_rows);
-    if (sp.j0 >= sp.j1 && split > 0) return;
+    make_plan(a, 16, kFewUnit, cum, scan);
+    if (blockIdx.x == 0)
+        for (int s = threadIdx.x; s <= a.n_seq; s += 256) a.plan[s] = cum[s];
+    const long all = cum[a.n_seq];
+    const int share = share_id();
+    const int used = shares_used(a, all);
+    if (share >= used) return;
+    long lo = share_start(all, share, used);
+    const long hi = share_start(all, share + 1, used);
+    int seq = 0;
+    while (lo < hi) {
+    const Span sp = next_span(a, cum, 16, kFewUnit, share, seq, lo, hi);
+    const int kvh = sp.kvh, tile = sp.tile, rows = sp.rows;
     const int rho = tile * 16 + n;
     const bool live = rho < rows;
     const long ld = (long)a.n_kv_heads * HD;
@@ -432,31 +572,32 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
     }
     uint4 qf[NC][QP];
     float scale;
-    load_q<HD, T>(a, sp, rho, kvh, live, qf, scale);
+    load_q<HD, T>(a, sp, rho, live, qf, scale);
     const uint64_t mask = live ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
-    f32x4 o[ND][SUMS];
+    f32x4 o[ND];
 #pragma unroll
-    for (int d = 0; d < ND; d++)
-#pragma unroll
-        for (int e = 0; e < SUMS; e++) o[d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
     float m = -INFINITY, l = 0.f;
     for (int jb = first; jb < sp.j1; jb += hop) {
         const bool more = jb + hop < sp.j1;
         f32x4 st[2][SUMS];
 #pragma unroll
-        for (int t = 0; t < 2; t++) {
+        for (int t = 0; t < 2; t++)
 #pragma unroll
             for (int e = 0; e < SUMS; e++) st[t][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int c2 = 0; c2 < NC; c2++) {
-                uint4 kf[KP];
-                if constexpr (KP == 1) {
-                    __builtin_memcpy(&kf[0], kr[t][c2], 16);
-                } else {
-                    Parts<T>::split_kv(kr[t][c2], kf);
-                }
-                Parts<T>::product(kf, qf[c2], st[t]);
+        for (int c2 = 0; c2 < NC; c2++) {
+            uint4 kf[2][KP];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                if constexpr (KP == 1)
+                    __builtin_memcpy(&kf[t][0], kr[t][c2], 16);
+                else
+                    Parts<T>::split_kv(kr[t][c2], kf[t]);
             }
+            const uint4* const q[1] = {qf[c2]};
+            f32x4* const to[2][1] = {{st[0]}, {st[1]}};
+            Parts<T>::template scores<2, 1>(kf, q, to);
         }
         // no row behind a key: only bad tables have such keys before j1
         const bool hole = __any(r[0] < 0 || r[1] < 0);
@@ -474,22 +615,22 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
         uint4 pf[QP];
         weights<T>(st, scale, hole || jb + kStep > min(sp.held, sp.j1), mask, jb, sp, bad, m, l, keep, pf);
 #pragma unroll
-        for (int d = 0; d < ND; d++) {
+        for (int d = 0; d < ND; d += 2) {
+            uint4 vf[2][KP];
 #pragma unroll
-            for (int e = 0; e < SUMS; e++) o[d][e] *= keep;
-            uint4 vf[KP];
-            if constexpr (KP == 1) {
+            for (int i = 0; i < 2; i++) {
+                o[d + i] *= keep;
                 T w[8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = vr[e >> 2][e & 3][d];
-                __builtin_memcpy(&vf[0], w, 16);
-            } else {
-                float w[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) w[e] = vr[e >> 2][e & 3][d];
-                Parts<T>::split_kv(w, vf);
+                for (int e = 0; e < 8; e++) w[e] = vr[e >> 2][e & 3][d + i];
+                if constexpr (KP == 1)
+                    __builtin_memcpy(&vf[i][0], w, 16);
+                else
+                    Parts<T>::split_kv(w, vf[i]);
             }
-            Parts<T>::product(vf, pf, o[d]);
+            const uint4* const p[1] = {pf};
+            f32x4* const to[2][1] = {{&o[d]}, {&o[d + 1]}};
+            Parts<T>::template product<2, 1>(vf, p, to);
         }
         if (more) {
             load_v(rn);
@@ -500,106 +641,123 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a, 
     }
     // the wave's sums, element (4 g + e) * ND + d of row n
     l = rows_sum(l);
-    float check = l;
 #pragma unroll
     for (int d = 0; d < ND; d++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const float y = Parts<T>::total(o[d], e);
-            os[wave][n][(4 * g + e) * ND + d] = y;
-            check = fmaf(y, 0.f, check);  // NaN if one of them is not finite
-        }
+        for (int e = 0; e < 4; e++)
+            os[wave][n][(4 * g + e) * ND + d] = o[d][e] * (1.f / Parts<T>::kUp);
     if (g == 0) {
         ms[wave][n] = m;
         ls[wave][n] = l;
     }
-    if (__any(live && !(fabsf(check) < INFINITY))) {
-        for (int t = 0; t < 16 && tile * 16 + t < rows; t++) {
-            float mc, lc, oc[HD / 64];
-            row_careful<HD, T>(a, sp, tile * 16 + t, kvh, wave, kFewWaves, mc, lc, oc);
-            ms[wave][t] = mc;
-            ls[wave][t] = lc;
-#pragma unroll
-            for (int e = 0; e < HD / 64; e++) os[wave][t][lane + 64 * e] = oc[e];
-        }
-    }
     __syncthreads();
     // thread: row threadIdx.x / 16, every 16th float4 of it
     const int t = threadIdx.x >> 4, u = threadIdx.x & 15;
-    if (tile * 16 + t >= rows) return;
-    float top = ms[0][t];
+    if (tile * 16 + t < rows) {
+        float top = ms[0][t];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; w++) top = fmaxf(top, ms[w][t]);
-    const float base = top == -INFINITY ? 0.f : top;
-    float f[kFewWaves], sum = 0.f;
-#pragma unroll
-    for (int w = 0; w < kFewWaves; w++) {
-        // a wave without a weight has nothing to add, whatever it holds
-        f[w] = ls[w][t] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[w][t] - base);
-        sum = fmaf(ls[w][t], f[w], sum);
-    }
-    const int ro = tile * 16 + t;
-    const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
-    const bool whole = a.nsplit == 1 && !a.outq8;
-    float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
-    if (!whole && u == 0) a.part_ml[orow * a.nsplit + split] = make_float2(top, sum);
-    const float by = !whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
-    for (int d = 4 * u; d < HD; d += 64) {
-        float y[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 1; w < kFewWaves; w++) top = fmaxf(top, ms[w][t]);
+        const float base = top == -INFINITY ? 0.f : top;
+        float f[kFewWaves], sum = 0.f;
 #pragma unroll
         for (int w = 0; w < kFewWaves; w++) {
-            if (ls[w][t] == 0.f) continue;
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = fmaf(os[w][t][d + e], f[w], y[e]);
+            // a wave without a weight has nothing to add, whatever it holds
+            f[w] = ls[w][t] == 0.f ? 0.f : __builtin_amdgcn_exp2f(ms[w][t] - base);
+            sum = fmaf(ls[w][t], f[w], sum);
         }
+        const bool whole = sp.slot < 0;
+        float* dst;
+        if (whole) {
+            dst = a.out + out_row(a, sp, tile * 16 + t) * HD;
+        } else {
+            dst = a.part + ((long)sp.slot * 16 + t) * HD;
+            if (u == 0) a.part_ml[sp.slot * 16 + t] = make_float2(top, sum);
+        }
+        const float by = !whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+        for (int d = 4 * u; d < HD; d += 64) {
+            float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-        for (int e = 0; e < 4; e++) dst[d + e] = y[e] * by;
+            for (int w = 0; w < kFewWaves; w++) {
+                if (ls[w][t] == 0.f) continue;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = fmaf(os[w][t][d + e], f[w], y[e]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) dst[d + e] = y[e] * by;
+        }
+    }
+    __syncthreads();
     }
 }
-// ---- more rows: the workgroup's four waves share each step's K and V through LDS,
+
+// ---- more rows: the workgroup's NW waves share each step's K and V through LDS,
 // split into operands once (by the thread that loaded them) and laid out as the
 // operands' fragments (64 lanes x 16 bytes), so every LDS access is 1 KiB in a row.
-// Wave w has the 16-row tiles w, w + 4, ... of the workgroup's 64 MW rows; with MW = 2
-// a fragment read from LDS feeds two tiles' products.  The next step's values are in
-// flight while this one is multiplied.
-template <int HD, class T, int MW>
-__global__ __launch_bounds__(256, 2) void k_attn_paged_many(PagedArgs a, int tiles) {
-    constexpr int NC = HD / 32, ND = HD / 16, DV = HD / 64, KP = Parts<T>::KP, QP = Parts<T>::QP,
-                  SUMS = Parts<T>::SUMS;
-    __shared__ uint4 kl[2 * NC * KP * 64];
-    __shared__ uint4 vl[ND * KP * 64];
-    __shared__ uint32_t holes;  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
+// Wave w has the 16-row tiles w and w + NW (MW = 2) of the workgroup's 16 NW MW rows; a
+// fragment read from LDS then feeds two tiles' products.  What a row tile costs
+// beside its products is the cache read again, so a tile is as large as registers allow:
+// 64 rows of 4 waves, two workgroups a CU, else 128 or 256 of 8 waves.  The next step's
+// values are in flight while this one is multiplied.
+constexpr int kManyUnit = kStep;
+
+// LDS of one step's fragments, and how many steps' fit beside each other (two: one
+// barrier a step instead of two) with the workgroups a CU is to hold.
+template <int HD, class T>
+constexpr int many_bytes() {
+    return (2 * (HD / 32) + HD / 16) * Parts<T>::KP * 1024;
+}
+template <int HD, class T, int NW>
+constexpr int many_bufs() {
+    return 2 * many_bytes<HD, T>() <= (NW == 8 ? 144 : 72) * 1024 ? 2 : 1;
+}
+
+template <int HD, class T, int NW, int MW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
+    constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
+                  SUMS = Parts<T>::SUMS, TR = 16 * NW * MW, NB = many_bufs<HD, T, NW>();
+    // a thread's part of a step: EK times 8 elements of a key's K; EV elements of 8 keys' V.
+    // 8 waves have both to do only from 128 elements a head up: at 64 the first four
+    // take K and the others V.
+    constexpr bool kHalves = HD == 64 && NW == 8;
+    constexpr int EK = kHalves ? 1 : 4 * HD / (64 * NW), EV = kHalves ? 1 : HD / 64 * 4 / NW;
+    __shared__ uint4 kl[NB][2 * NC * KP * 64];
+    __shared__ uint4 vl[NB][ND * KP * 64];
+    __shared__ uint32_t holes[NB];  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
+    __shared__ long cum[kPlanSeqs + 1], scan[4];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
-    const int per = (a.n_kv_heads * a.nsplit + 7) & ~7;  // XCDs as in k_attn_paged_few
-    const int xcd = blockIdx.x & 7, rest = blockIdx.x >> 3;
-    const int tile = rest % tiles, cc = (rest / tiles) * 8 + xcd;
-    const int x = cc % per;
-    if (x >= a.n_kv_heads * a.nsplit) return;
-    const int kvh = x / a.nsplit, split = x % a.nsplit;
-    Span sp;
-    sp.s = cc / per;
-    const SeqLen len = seq_len(a.len, a.n_tok, a.max_tok, sp.s, a.table_ld, a.page_shift);
-    sp.held = len.held;
-    sp.tok = len.tok;
-    sp.table = a.table + (long)sp.s * a.table_ld;
-    const int total = sp.held + sp.tok, rows = sp.tok * G, row0 = tile * 64 * MW;
-    if (row0 >= rows) return;
-    sp.j0 = split * a.split_rows;
-    sp.j1 = split + 1 == a.nsplit ? total : min(total, sp.j0 + a.split_rows);
-    if (sp.j0 >= sp.j1 && split > 0) return;
+    make_plan(a, TR, kManyUnit, cum, scan);
+    if (blockIdx.x == 0)
+        for (int s = t; s <= a.n_seq; s += 64 * NW) a.plan[s] = cum[s];
+    const long all = cum[a.n_seq];
+    const int share = share_id();
+    const int used = shares_used(a, all);
+    if (share >= used) return;
+    long lo = share_start(all, share, used);
+    const long hi = share_start(all, share + 1, used);
+    int seq = 0;
+    while (lo < hi) {
+    const Span sp = next_span(a, cum, TR, kManyUnit, share, seq, lo, hi);
+    const int kvh = sp.kvh, rows = sp.rows, row0 = sp.tile * TR;
     const long ld = (long)a.n_kv_heads * HD;
 
-    // this thread's part of a step: K: key t & 15 of a tile, 8 elements; V: the 8 keys of
-    // group `wave`, DV elements
-    T kr[DV][8], vr[8][DV];
+    const bool do_k = !kHalves || wave < 4, do_v = !kHalves || wave >= 4;
+    const int kt = t & 255;  // with kHalves; else t
+    const int vg = wave & 3, vd = kHalves ? lane : (wave >> 2) * (64 * EV) + lane * EV;
+    T kr[EK][8], vr[8][EV];
     int pg[2];  // table entries of keys t & 15 of both tiles (as in k_attn_paged_few)
     auto pages_of = [&](int jb) {
 #pragma unroll
         for (int tt = 0; tt < 2; tt++)
             pg[tt] = kv_page(min(jb + 16 * tt + n, sp.j1 - 1), sp.table, a.table_ld, a.page_shift);
     };
-    uint32_t bad = 0, bad_next = 0;
+    uint32_t bad_next = 0;
+    // K unit p of the thread: key n of tile tt, elements 8 j ..
+    auto k_unit = [&](int p, int& tt, int& j) {
+        const int u = ((kHalves ? kt : t) >> 4) + 4 * NW * p;
+        tt = u / (HD / 8);
+        j = u % (HD / 8);
+    };
     auto fetch = [&](int jb) {
         int krow[2], vrow[8];
 #pragma unroll
@@ -608,53 +766,65 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged_many(PagedArgs a, int til
                                       a.page_shift);
 #pragma unroll
         for (int e = 0; e < 8; e++)
-            vrow[e] = __builtin_amdgcn_readlane(krow[e >> 2], 4 * wave + (e & 3));
+            vrow[e] = __builtin_amdgcn_readlane(krow[e >> 2], 4 * vg + (e & 3));
         const T* kb = static_cast<const T*>(a.k) + kvh * HD;
-        const T* vb = static_cast<const T*>(a.v) + kvh * HD + lane * DV;
+        const T* vb = static_cast<const T*>(a.v) + kvh * HD + vd;
+        if (do_k) {
 #pragma unroll
-        for (int p = 0; p < DV; p++) {
-            const int u = (t >> 4) + 16 * p, tt = u / (HD / 8), j = u % (HD / 8);
-            const int row = HD >= 128 ? krow[p / (HD / 128 ? HD / 128 : 1)] : (tt ? krow[1] : krow[0]);
-            __builtin_memcpy(kr[p], __builtin_assume_aligned(kb + (long)max(row, 0) * ld + 8 * j, 16),
-                             8 * sizeof(T));
+            for (int p = 0; p < EK; p++) {
+                int tt, j;
+                k_unit(p, tt, j);
+                __builtin_memcpy(
+                    kr[p],
+                    __builtin_assume_aligned(kb + (long)max(tt ? krow[1] : krow[0], 0) * ld + 8 * j, 16),
+                    8 * sizeof(T));
+            }
         }
         bad_next = 0;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            bad_next |= (uint32_t)(vrow[e] < 0) << e;
-            __builtin_memcpy(vr[e],
-                             __builtin_assume_aligned(vb + (long)max(vrow[e], 0) * ld, DV * sizeof(T)),
-                             DV * sizeof(T));
+        for (int e = 0; e < 8; e++) bad_next |= (uint32_t)(vrow[e] < 0) << e;
+        if (do_v) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                __builtin_memcpy(
+                    vr[e], __builtin_assume_aligned(vb + (long)max(vrow[e], 0) * ld, EV * sizeof(T)),
+                    EV * sizeof(T));
         }
     };
-    auto put = [&] {  // split what was fetched into LDS
+    auto put = [&](int buf) {  // split what was fetched into LDS
+        if (do_k) {
 #pragma unroll
-        for (int p = 0; p < DV; p++) {
-            const int u = (t >> 4) + 16 * p, tt = u / (HD / 8), j = u % (HD / 8);
-            uint4 f[KP];
-            if constexpr (KP == 1)
-                __builtin_memcpy(&f[0], kr[p], 16);
-            else
-                Parts<T>::split_kv(kr[p], f);
+            for (int p = 0; p < EK; p++) {
+                int tt, j;
+                k_unit(p, tt, j);
+                uint4 f[KP];
+                if constexpr (KP == 1)
+                    __builtin_memcpy(&f[0], kr[p], 16);
+                else
+                    Parts<T>::split_kv(kr[p], f);
 #pragma unroll
-            for (int q = 0; q < KP; q++)
-                kl[((tt * NC + j / 4) * KP + q) * 64 + (j & 3) * 16 + (t & 15)] = f[q];
+                for (int q = 0; q < KP; q++)
+                    kl[buf][((tt * NC + j / 4) * KP + q) * 64 + (j & 3) * 16 + n] = f[q];
+            }
         }
+        if (do_v) {
 #pragma unroll
-        for (int e = 0; e < DV; e++) {
-            const int d = lane * DV + e;
-            T w[8];
+            for (int e = 0; e < EV; e++) {
+                const int d = vd + e;
+                T w[8];
 #pragma unroll
-            for (int r = 0; r < 8; r++) w[r] = vr[r][e];
-            uint4 f[KP];
-            if constexpr (KP == 1)
-                __builtin_memcpy(&f[0], w, 16);
-            else
-                Parts<T>::split_kv(w, f);
+                for (int r = 0; r < 8; r++) w[r] = vr[r][e];
+                uint4 f[KP];
+                if constexpr (KP == 1)
+                    __builtin_memcpy(&f[0], w, 16);
+                else
+                    Parts<T>::split_kv(w, f);
 #pragma unroll
-            for (int q = 0; q < KP; q++) vl[((d >> 4) * KP + q) * 64 + wave * 16 + (d & 15)] = f[q];
+                for (int q = 0; q < KP; q++)
+                    vl[buf][((d >> 4) * KP + q) * 64 + vg * 16 + (d & 15)] = f[q];
+            }
         }
-        if (lane == 0) reinterpret_cast<uint8_t*>(&holes)[wave] = (uint8_t)bad_next;
+        if (lane == 0 && wave < 4) reinterpret_cast<uint8_t*>(&holes[buf])[wave] = (uint8_t)bad_next;
     };
 
     pages_of(sp.j0);
@@ -663,160 +833,200 @@ __global__ __launch_bounds__(256, 2) void k_attn_paged_many(PagedArgs a, int til
 
     uint4 qf[MW][NC][QP];
     float scale[MW], m[MW], l[MW];
-    uint64_t mask[MW];
     bool act[MW], live[MW];
-    f32x4 o[MW][ND][SUMS];
+    f32x4 o[MW][ND];
 #pragma unroll
     for (int w = 0; w < MW; w++) {
-        const int rho = row0 + (wave + 4 * w) * 16 + n;
-        act[w] = row0 + (wave + 4 * w) * 16 < rows;
+        const int rho = row0 + (wave + NW * w) * 16 + n;
+        act[w] = row0 + (wave + NW * w) * 16 < rows;
         live[w] = rho < rows;
-        load_q<HD, T>(a, sp, rho, kvh, live[w], qf[w], scale[w]);
-        mask[w] = live[w] ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
+        load_q<HD, T>(a, sp, rho, live[w], qf[w], scale[w]);
         m[w] = -INFINITY;
         l[w] = 0.f;
 #pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < SUMS; e++) o[w][d][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int d = 0; d < ND; d++) o[w][d] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
+    put(0);
+    if (sp.j0 + kStep < sp.j1) {
+        fetch(sp.j0 + kStep);
+        pages_of(sp.j0 + 2 * kStep);
+    }
+    int buf = 0;
     for (int jb = sp.j0; jb < sp.j1; jb += kStep) {
-        put();
-        if (jb + kStep < sp.j1) {
-            fetch(jb + kStep);
-            pages_of(jb + 2 * kStep);
-        }
         __syncthreads();
-        if (act[0]) {
-            f32x4 st[MW][2][SUMS];
+        // M row tiles' products side by side; with one, two key tiles' or elements' tiles
+        auto multiply = [&](auto tiles_of_wave) {
+            constexpr int M = decltype(tiles_of_wave)::value, NA = 3 - M;
+            f32x4 st[M][2][SUMS];
 #pragma unroll
-            for (int w = 0; w < MW; w++)
+            for (int w = 0; w < M; w++)
 #pragma unroll
                 for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                     for (int e = 0; e < SUMS; e++) st[w][tt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int tt = 0; tt < 2; tt++)
+            for (int c = 0; c < NC; c++) {
+                const uint4* q[M];
 #pragma unroll
-                for (int c = 0; c < NC; c++) {
-                    uint4 f[KP];
+                for (int w = 0; w < M; w++) q[w] = qf[w][c];
 #pragma unroll
-                    for (int q = 0; q < KP; q++) f[q] = kl[((tt * NC + c) * KP + q) * 64 + lane];
+                for (int tt = 0; tt < 2; tt += NA) {
+                    uint4 f[NA][KP];
+                    f32x4* to[NA][M];
 #pragma unroll
-                    for (int w = 0; w < MW; w++)
-                        if (w == 0 || act[w]) Parts<T>::product(f, qf[w][c], st[w][tt]);
+                    for (int i = 0; i < NA; i++) {
+#pragma unroll
+                        for (int p = 0; p < KP; p++)
+                            f[i][p] = kl[buf][(((tt + i) * NC + c) * KP + p) * 64 + lane];
+#pragma unroll
+                        for (int w = 0; w < M; w++) to[i][w] = st[w][tt + i];
+                    }
+                    Parts<T>::template scores<NA, M>(f, q, to);
                 }
-            const uint32_t hole = holes;
-            bad = (hole >> (8 * g)) & 255;
-            uint4 pf[MW][QP];
+            }
+            const uint32_t hole = holes[buf], bad = (hole >> (8 * g)) & 255;
+            uint4 pf[M][QP];
+            const uint4* p[M];
 #pragma unroll
-            for (int w = 0; w < MW; w++) {
-                if (w > 0 && !act[w]) continue;
+            for (int w = 0; w < M; w++) {
                 float keep;
-                weights<T>(st[w], scale[w], hole || jb + kStep > min(sp.held, sp.j1), mask[w], jb, sp,
-                           bad, m[w], l[w], keep, pf[w]);
+                const bool masked = hole || jb + kStep > min(sp.held, sp.j1);
+                uint64_t mask = 0;  // wanted in few steps: not kept
+                if (masked && live[w]) {
+                    const int i = (row0 + (wave + NW * w) * 16 + n) / G;
+                    mask = seen_mask(a, (long)sp.s * a.max_tok + i, i);
+                }
+                weights<T>(st[w], scale[w], masked, mask, jb, sp, bad, m[w], l[w], keep, pf[w]);
+                p[w] = pf[w];
+                if (__any(keep != 1.f)) {  // seldom after the first steps
 #pragma unroll
-                for (int d = 0; d < ND; d++)
-#pragma unroll
-                    for (int e = 0; e < SUMS; e++) o[w][d][e] *= keep;
+                    for (int d = 0; d < ND; d++) o[w][d] *= keep;
+                }
             }
 #pragma unroll
-            for (int d = 0; d < ND; d++) {
-                uint4 f[KP];
+            for (int d = 0; d < ND; d += NA) {
+                uint4 f[NA][KP];
+                f32x4* to[NA][M];
 #pragma unroll
-                for (int q = 0; q < KP; q++) f[q] = vl[(d * KP + q) * 64 + lane];
+                for (int i = 0; i < NA; i++) {
 #pragma unroll
-                for (int w = 0; w < MW; w++)
-                    if (w == 0 || act[w]) Parts<T>::product(f, pf[w], o[w][d]);
+                    for (int q = 0; q < KP; q++) f[i][q] = vl[buf][((d + i) * KP + q) * 64 + lane];
+#pragma unroll
+                    for (int w = 0; w < M; w++) to[i][w] = &o[w][d + i];
+                }
+                Parts<T>::template product<NA, M>(f, p, to);
+            }
+        };
+        if (MW == 2 && act[MW - 1])
+            multiply(std::integral_constant<int, MW>());
+        else if (act[0])
+            multiply(std::integral_constant<int, 1>());
+        if (NB == 1) __syncthreads();
+        if (jb + kStep < sp.j1) {
+            buf = NB == 1 ? 0 : buf ^ 1;
+            put(buf);
+            if (jb + 2 * kStep < sp.j1) {
+                fetch(jb + 2 * kStep);
+                pages_of(jb + 3 * kStep);
             }
         }
-        __syncthreads();
     }
-    const bool whole = a.nsplit == 1 && !a.outq8;
+    __syncthreads();
+    const bool whole = sp.slot < 0;
 #pragma unroll
     for (int w = 0; w < MW; w++) {
         if (!act[w]) continue;
         l[w] = rows_sum(l[w]);
-        float check = l[w];
-#pragma unroll
-        for (int d = 0; d < ND; d++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) check = fmaf(Parts<T>::total(o[w][d], e), 0.f, check);
-        const int tile0 = row0 + (wave + 4 * w) * 16;
-        if (__any(live[w] && !(fabsf(check) < INFINITY))) {
-            for (int i = 0; i < 16 && tile0 + i < rows; i++) {
-                float mc, lc, oc[HD / 64];
-                row_careful<HD, T>(a, sp, tile0 + i, kvh, 0, 1, mc, lc, oc);
-                const int ro = tile0 + i;
-                const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
-                float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
-                if (!whole && lane == 0) a.part_ml[orow * a.nsplit + split] = make_float2(mc, lc);
-                for (int e = 0; e < HD / 64; e++)
-                    dst[lane + 64 * e] = !whole ? oc[e] : (lc == 0.f ? 0.f : oc[e] / lc);
-            }
-            continue;
-        }
+        const int in = (wave + NW * w) * 16;  // the tile's first row within the workgroup's
         if (!live[w]) continue;
-        const int ro = tile0 + n;
-        const long orow = ((long)sp.s * a.max_tok + ro / G) * a.n_heads + kvh * G + ro % G;
-        float* dst = whole ? a.out + orow * HD : a.part + (orow * a.nsplit + split) * HD;
-        if (!whole && g == 0) a.part_ml[orow * a.nsplit + split] = make_float2(m[w], l[w]);
-        const float by = !whole ? 1.f : (l[w] == 0.f ? 0.f : 1.f / l[w]);
+        float* dst = whole ? a.out + out_row(a, sp, row0 + in + n) * HD
+                           : a.part + ((long)sp.slot * TR + in + n) * HD;
+        if (!whole && g == 0) a.part_ml[sp.slot * TR + in + n] = make_float2(m[w], l[w]);
+        const float by = (!whole ? 1.f : (l[w] == 0.f ? 0.f : 1.f / l[w])) / Parts<T>::kUp;
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             f32x4_a4 y;
 #pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = Parts<T>::total(o[w][d], e) * by;
+            for (int e = 0; e < 4; e++) y[e] = o[w][d][e] * by;
             *reinterpret_cast<f32x4_a4*>(dst + 16 * d + 4 * g) = y;
         }
     }
+    }
 }
 
-// One wave a query row and head: the splits' sums brought to one base and added
-// in their order, divided by the weights' sum.  Lane j has split j's m and l (at most
-// 64 splits), so one load's latency covers them all.
-template <int HD>
-__global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a) {
+// One wave a query row and head.  Where its part lies in several shares, their sums are
+// brought to one base and added in their order, and divided by the weights' sum (lane j
+// has share j's m and l, so one load's latency covers 64 of them); a whole part's row
+// is read back.  A row that is not finite is done again with care.
+template <int HD, class T>
+__global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows, int unit) {
     constexpr int E = HD / 64, U = 8;
     const int lane = threadIdx.x & 63;
-    const long w = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const long w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
     if (w >= (long)a.n_seq * a.max_tok * a.n_heads) return;
-    const long row = w / a.n_heads;
-    const int s = (int)(row / a.max_tok);
+    const int h = (int)(w % a.n_heads), i = (int)(w / a.n_heads % a.max_tok);
+    const int s = (int)(w / a.n_heads / a.max_tok), G = a.n_heads / a.n_kv_heads;
+    const long all = a.plan[a.n_seq], before = a.plan[s];
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
-    if ((int)(row % a.max_tok) >= n.tok) return;
-    const int used = __builtin_amdgcn_readfirstlane(
-        min(a.nsplit, (n.held + n.tok + a.split_rows - 1) / a.split_rows));
-    const float2 ml = lane < used ? a.part_ml[w * a.nsplit + lane] : make_float2(-INFINITY, 0.f);
-    const float* p = a.part + w * a.nsplit * HD + lane * E;
-    const float top = wave_max(ml.x);
-    const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - (top == -INFINITY ? 0.f : top));
-    const float l = wave_sum(ml.y * f);
-    float o[E];
-#pragma unroll
-    for (int e = 0; e < E; e++) o[e] = 0.f;
-    for (int j0 = 0; j0 < used; j0 += U) {
-        float v[U][E];
-#pragma unroll
-        for (int j = 0; j < U; j++)
-#pragma unroll
-            for (int e = 0; e < E; e++) v[j][e] = p[(long)min(j0 + j, used - 1) * HD + e];
-#pragma unroll
-        for (int j = 0; j < U; j++) {
-            const float fj = j0 + j < used ? __uint_as_float(__builtin_amdgcn_readlane(
-                                                 __float_as_uint(f), (j0 + j) & 63))
-                                           : 0.f;
-            if (fj == 0.f) continue;
-#pragma unroll
-            for (int e = 0; e < E; e++) o[e] = fmaf(v[j][e], fj, o[e]);
-        }
-    }
+    if (i >= n.tok) return;
+    const SeqWork sw = seq_work(n, G, tile_rows, unit);
+    const int rho = i * G + h % G, tile = rho / tile_rows;
+    const long p0 = before + ((long)(h / G) * sw.tiles + tile) * sw.units;
+    const int shares = shares_used(a, all);
+    const int w1 = __builtin_amdgcn_readfirstlane(share_of(all, p0, shares));
+    const int w2 = __builtin_amdgcn_readfirstlane(share_of(all, p0 + sw.units - 1, shares));
     float* dst = a.out + w * HD + lane * E;
-    const float by = l == 0.f ? 0.f : 1.f / l;
+    float o[E], l = 1.f;
+    if (w1 == w2) {
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        o[e] *= by;
-        dst[e] = o[e];
+        for (int e = 0; e < E; e++) o[e] = dst[e];
+    } else {
+        const int at = rho % tile_rows, used = w2 - w1 + 1;
+        // the part's first share has it last, the others first
+        auto slot = [&](int j) { return (long)(j == 0 ? 2 * w1 + 1 : 2 * (w1 + j)) * tile_rows + at; };
+        const float2 none = make_float2(-INFINITY, 0.f);
+        float top = -INFINITY;
+        for (int j = lane; j < used; j += 64) top = fmaxf(top, a.part_ml[slot(j)].x);
+        top = wave_max(top);
+        const float base = top == -INFINITY ? 0.f : top;
+        l = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] = 0.f;
+        for (int b = 0; b < used; b += 64) {
+            const float2 ml = b + lane < used ? a.part_ml[slot(b + lane)] : none;
+            const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - base);
+            l += wave_sum(ml.y * f);
+            const int here = min(64, used - b);
+            for (int j0 = 0; j0 < here; j0 += U) {
+                float v[U][E];
+#pragma unroll
+                for (int j = 0; j < U; j++)
+#pragma unroll
+                    for (int e = 0; e < E; e++)
+                        v[j][e] = a.part[slot(b + min(j0 + j, here - 1)) * HD + lane * E + e];
+#pragma unroll
+                for (int j = 0; j < U; j++) {
+                    const float fj = j0 + j < here ? __uint_as_float(__builtin_amdgcn_readlane(
+                                                         __float_as_uint(f), (j0 + j) & 63))
+                                                   : 0.f;
+                    if (fj == 0.f) continue;  // no weight there, whatever it holds
+#pragma unroll
+                    for (int e = 0; e < E; e++) o[e] = fmaf(v[j][e], fj, o[e]);
+                }
+            }
+        }
+        const float by = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] *= by;
+    }
+    float check = l * 0.f;
+#pragma unroll
+    for (int e = 0; e < E; e++) check = fmaf(o[e], 0.f, check);
+    const bool again = __any(check != 0.f);
+    if (again) row_careful<HD, T>(a, s, i, h, o);
+    if (again || w1 != w2) {
+#pragma unroll
+        for (int e = 0; e < E; e++) dst[e] = o[e];
     }
     if (a.outq8) {
         // a block's 32 values are in 32 / E neighbouring lanes
@@ -1116,30 +1326,41 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
     len_out[s] = kv_len(len[s], table_ld, page_shift) + n;
 }
 
-// Query rows of a KV head that a workgroup takes (attn_paged_plan has the rule).
+// Query rows of a KV head that a workgroup takes: the fewest that hold them all, so that
+// the cache is read once; with 256 elements a head 256 rows' sums do not fit.
 int tile_rows(int rows, int head_dim) {
     if (rows <= 16) return 16;
-    return rows <= 64 || head_dim == 256 ? 64 : 128;
+    if (rows <= 64) return 64;
+    return rows <= 128 || head_dim == 256 ? 128 : 256;
 }
 
 template <int HD, class T>
 hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
-    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, HD);
-    const int tiles = (rows + tr - 1) / tr;
-    const long per = (a.n_kv_heads * a.nsplit + 7) & ~7;
-    const unsigned wgs = (unsigned)(per * a.n_seq * tiles);
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), HD);
     if (tr == 16) {
-        k_attn_paged_few<HD, T><<<wgs, 64 * kFewWaves, 0, st>>>(a, tiles);
+        k_attn_paged_few<HD, T><<<a.shares, 64 * kFewWaves, 0, st>>>(a);
     } else if (tr == 64) {
-        k_attn_paged_many<HD, T, 1><<<wgs, 256, 0, st>>>(a, tiles);
+        k_attn_paged_many<HD, T, 4, 1><<<a.shares, 256, 0, st>>>(a);
+    } else if (tr == 128) {
+        k_attn_paged_many<HD, T, 8, 1><<<a.shares, 512, 0, st>>>(a);
     } else {
-        if constexpr (HD < 256) k_attn_paged_many<HD, T, 2><<<wgs, 256, 0, st>>>(a, tiles);
+        if constexpr (HD < 256) k_attn_paged_many<HD, T, 8, 2><<<a.shares, 512, 0, st>>>(a);
     }
-    if (a.nsplit > 1 || a.outq8) {
-        const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
-        k_attn_paged_join<HD><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a);
-    }
+    const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
+    k_attn_paged_join<HD, T><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(
+        a, tr, tr == 16 ? kFewUnit : kManyUnit);
     return hipGetLastError();
+}
+
+hipError_t attn_types(const PagedArgs& a, int kv_type, int head_dim, hipStream_t st) {
+    if (kv_type == AXF_TYPE_F16) {
+        if (head_dim == 64) return attn_launch<64, _Float16>(a, st);
+        if (head_dim == 128) return attn_launch<128, _Float16>(a, st);
+        return attn_launch<256, _Float16>(a, st);
+    }
+    if (head_dim == 64) return attn_launch<64, float>(a, st);
+    if (head_dim == 128) return attn_launch<128, float>(a, st);
+    return attn_launch<256, float>(a, st);
 }
 
 template <int HD, class T>
@@ -1151,34 +1372,46 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 
 }  // namespace
 
-void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
-    (void)kv_type;
+// Workgroups of the launch: as many as run at once (two of 4 waves a CU, one of 8), or as
+// few as have a unit each by the caller's estimate of the lengths.
+void attn_paged_plan(PagedArgs& a, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
     const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, head_dim);
-    const long parts = (long)a.n_seq * a.n_kv_heads * ((rows + tr - 1) / tr);
-    const long unit = tr == 16 ? kStep * kFewWaves : 2 * kStep;
-    long split = longest * parts / (tr == 16 ? 1024 : 768);
-    split = split < unit ? unit : (split + unit - 1) / unit * unit;
-    while ((longest + split - 1) / split > 64) split += unit;  // the join's lanes
-    a.split_rows = (int)split;
-    a.nsplit = (int)((longest + split - 1) / split);
+    const long seqs = a.n_seq < kPlanSeqs ? a.n_seq : kPlanSeqs;
+    const long units = (longest + (tr == 16 ? kFewUnit : kManyUnit) - 1) /
+                       (tr == 16 ? kFewUnit : kManyUnit) * seqs * a.n_kv_heads * ((rows + tr - 1) / tr);
+    const long most = tr > 64 ? 256 : 512;
+    const long shares = units < most ? units : most;
+    a.shares = (int)((shares + 7) & ~7L);
 }
 
 size_t attn_paged_scratch(const PagedArgs& a, int head_dim) {
-    if (a.nsplit == 1 && !a.outq8) return 0;
-    return (size_t)a.n_seq * a.max_tok * a.n_heads * a.nsplit * (head_dim + 2) * 4;
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim);
+    return (kPlanSeqs + 1) * sizeof(long) + (size_t)2 * a.shares * tr * (head_dim + 2) * 4 + 16;
 }
 
-hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, hipStream_t st) {
-    if (kv_type == AXF_TYPE_F16) {
-        if (head_dim == 64) return attn_launch<64, _Float16>(a, st);
-        if (head_dim == 128) return attn_launch<128, _Float16>(a, st);
-        return attn_launch<256, _Float16>(a, st);
+hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, void* scratch,
+                             hipStream_t st) {
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim);
+    for (int s = 0; s < a.n_seq; s += kPlanSeqs) {
+        PagedArgs b = a;
+        const long row = (long)s * a.max_tok;
+        b.n_seq = a.n_seq - s < kPlanSeqs ? a.n_seq - s : kPlanSeqs;
+        b.q += row * a.q_ld;
+        b.table += (long)s * a.table_ld;
+        b.len += s;
+        if (b.n_tok) b.n_tok += s;
+        if (b.mask) b.mask += row;
+        if (b.pos) b.pos += row;
+        b.out += row * a.n_heads * head_dim;
+        if (b.outq8) b.outq8 += row * a.n_heads * (head_dim / 32) * Q8_0_BYTES;
+        b.part = static_cast<float*>(scratch);
+        b.part_ml = reinterpret_cast<float2*>(b.part + 2L * a.shares * tr * head_dim);
+        b.plan = reinterpret_cast<long*>(b.part_ml + 2L * a.shares * tr);
+        if (hipError_t e = attn_types(b, kv_type, head_dim, st); e != hipSuccess) return e;
     }
-    if (head_dim == 64) return attn_launch<64, float>(a, st);
-    if (head_dim == 128) return attn_launch<128, float>(a, st);
-    return attn_launch<256, float>(a, st);
+    return hipSuccess;
 }
 
 hipError_t launch_kv_store(const KvStoreArgs& a, int kv_type, int head_dim, hipStream_t st) {
