@@ -345,8 +345,8 @@ struct PagedArgs {
     float2* part_ml;  // [share][2][tile rows]: their maximum (base 2) and weight sum
     long* plan;       // units before each sequence
 };
-void attn_paged_plan(PagedArgs& a, int head_dim, int max_len);
-size_t attn_paged_scratch(const PagedArgs& a, int head_dim);
+void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len);
+size_t attn_paged_scratch(const PagedArgs& a, int kv_type, int head_dim);
 hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, void* scratch,
                              hipStream_t st);
 struct KvStoreArgs {

@@ -191,9 +191,9 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
     a.page_shift = page_shift(kv);
     a.out = out;
     a.outq8 = static_cast<uint8_t*>(outq8);
-    attn_paged_plan(a, kv->head_dim, max_len);
+    attn_paged_plan(a, kv->type, kv->head_dim, max_len);
     void* scratch = nullptr;
-    int rc = ctx_scratch(ctx, attn_paged_scratch(a, kv->head_dim), &scratch);
+    int rc = ctx_scratch(ctx, attn_paged_scratch(a, kv->type, kv->head_dim), &scratch);
     if (rc) return rc;
     AXF_HIP(launch_attn_paged(a, kv->type, kv->head_dim, scratch, ctx->stream));
     return AXF_OK;

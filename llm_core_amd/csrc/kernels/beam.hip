@@ -10,8 +10,8 @@
 //   1. k_beam_part: a workgroup takes a chunk of a row: its maximum m, sum of
 //      exp(x - m) and its n_out largest (logit, lower token first) keys.
 //   2. k_beam_merge: a workgroup a sequence joins the chunks' sums to each beam's
-//      lse, turns the keys into scores and merges the chunks' sorted lists to
-//      the n_out best.
+//      lse, turns the keys into scores and picks the n_out best of the chunks' sorted
+//      lists.
 #include "common.hpp"
 
 namespace axf {
@@ -259,68 +259,164 @@ __device__ __forceinline__ Cand merge64(Cand a, Cand b) {
     return a;
 }
 
+// The k-th largest score of the wave's 64 (scores may be equal), or 0 with fewer.
+__device__ __forceinline__ uint64_t kth_score(uint64_t s, int k) {
+    const uint32_t hi = (uint32_t)(s >> 32), lo = (uint32_t)s;
+    uint32_t t = 0;
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t c = t | (1u << b);
+        if (__popcll(__ballot(hi >= c)) >= k) t = c;
+    }
+    const int above = __popcll(__ballot(hi > t));
+    const bool same = hi == t;
+    uint32_t v = 0;
+    for (int b = 31; b >= 0; b--) {
+        const uint32_t c = v | (1u << b);
+        if (__popcll(__ballot(same && lo >= c)) >= k - above) v = c;
+    }
+    return ((uint64_t)t << 32) | v;
+}
+
+constexpr int kMergeCap = 512;  // candidates ranked at once
+
+// The chunks' lists of one sequence.  Their heads come first: a score that n_out heads
+// reach bounds what can be among the n_out best, which leaves few lists and few of
+// their entries (some n_out to 3 n_out candidates, ranked by counting), so that the
+// rest is never read.  Many equal scores may pass the bound; then the lists are
+// merged in turn, each wave a share of them.
 __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
     BeamArgs a, int chunks, const uint64_t* __restrict__ keys, const float* __restrict__ ms,
     const double* __restrict__ ss) {
     constexpr int NW = kMergeThreads / 64;
-    __shared__ double lse[64];
+    __shared__ double lse[64], cums[64];
+    __shared__ int over[64];
     __shared__ Cand half[NW / 2][64];
+    __shared__ Cand list[kMergeCap];
+    __shared__ uint64_t bound[NW];
+    __shared__ int count;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const size_t row0 = (size_t)blockIdx.x * a.n_beams;
+    const int lists = a.n_beams * chunks;
+    keys += row0 * chunks * a.n_out;
+    if (t == 0) count = 0;
+    if (t < a.n_beams) {
+        cums[t] = (double)a.cum[row0 + t];
+        over[t] = a.done && a.done[row0 + t] != 0;
+    }
+    // the first round's heads are in flight while the sums are joined
+    const uint64_t head0 = t < lists ? keys[(size_t)t * a.n_out] : 0;
     for (int b = wave; b < a.n_beams; b += NW) {
         const float* mr = ms + (row0 + b) * chunks;
         const double* sr = ss + (row0 + b) * chunks;
-        float m = -INFINITY;
-        for (int c = lane; c < chunks; c += 64) m = fmaxf(m, mr[c]);
+        float m0 = -INFINITY, m = -INFINITY;
+        double s0 = 0.0, s = 0.0;
+        if (lane < chunks) {
+            m0 = mr[lane];
+            s0 = sr[lane];
+        }
+        m = m0;
+        for (int c = lane + 64; c < chunks; c += 64) m = fmaxf(m, mr[c]);
         m = wave_max(m);
         const double top = m == -INFINITY ? 0.0 : (double)m;
-        double s = 0.0;
-        for (int c = lane; c < chunks; c += 64) s += sr[c] * exp_neg((double)mr[c] - top);
+        s = s0 * exp_neg((double)m0 - top);
+        for (int c = lane + 64; c < chunks; c += 64) s += sr[c] * exp_neg((double)mr[c] - top);
         s = wave_sum64(s);
         // all logits -inf: log 0, and every score -inf - -inf
         if (lane == 0) lse[b] = top + log(s);
     }
     __syncthreads();
-    Cand acc = {0, 0};
-    for (int l = wave; l < a.n_beams * chunks; l += NW) {
+    // list l's entry with key k (entry 0 of a finished beam's first list: its one)
+    auto cand_of = [&](int l, uint64_t k, int rank) {
         const int b = l / chunks;
-        const bool over = a.done && a.done[row0 + b] != 0;
         Cand c = {0, 0};
-        const double cum = (double)a.cum[row0 + b];
-        if (over) {
-            if (l % chunks == 0 && lane == 0 && cum > -INFINITY)
-                c = {ordered64(cum), ((uint64_t)(63 - b) << 58) | (uint64_t)(0x3ffffff - a.eos)};
-        } else if (lane < a.n_out) {
-            const uint64_t k = keys[(row0 * chunks + l) * a.n_out + lane];
+        const uint64_t mine = (uint64_t)(63 - b) << 58;
+        if (over[b]) {
+            if (l % chunks == 0 && rank == 0 && cums[b] > -INFINITY)
+                c = {ordered64(cums[b]), mine | (uint64_t)(0x3ffffff - a.eos)};
+        } else if (k) {
             const uint32_t x = (uint32_t)(k >> 32);
-            const double score = cum + ((double)unordered32(x) - lse[b]);
-            if (k && score > -INFINITY)
-                c = {ordered64(score), ((uint64_t)(63 - b) << 58) | ((uint64_t)x << 26) |
-                                           (uint64_t)(0x3ffffff - ~(uint32_t)k)};
+            const double score = cums[b] + ((double)unordered32(x) - lse[b]);
+            if (score > -INFINITY)
+                c = {ordered64(score),
+                     mine | ((uint64_t)x << 26) | (uint64_t)(0x3ffffff - ~(uint32_t)k)};
         }
+        return c;
+    };
+    uint64_t head = 0;
+    for (int l = t; l < lists; l += kMergeThreads) {
+        const uint64_t s = cand_of(l, l == t ? head0 : keys[(size_t)l * a.n_out], 0).score;
+        head = s > head ? s : head;
+    }
+    const uint64_t mine = kth_score(head, a.n_out);
+    if (lane == 0) bound[wave] = mine;
+    __syncthreads();
+    uint64_t least = 1;
+#pragma unroll
+    for (int w = 0; w < NW; w++) least = bound[w] > least ? bound[w] : least;
+    // the lists whose head reaches it, a wave's lanes over one list's entries
+    for (int l0 = wave * 64; l0 < lists; l0 += kMergeThreads) {
+        const int l = l0 + lane;
+        const bool in = l < lists &&
+                        cand_of(l, l == t ? head0 : keys[(size_t)l * a.n_out], 0).score >= least;
+        for (uint64_t left = __ballot(in); left; left &= left - 1) {
+            const int pick = l0 + __builtin_ctzll(left);
+            Cand c = {0, 0};
+            if (lane < a.n_out) c = cand_of(pick, keys[(size_t)pick * a.n_out + lane], lane);
+            const uint64_t reach = __ballot(c.score >= least);
+            int at = 0;
+            if (lane == 0) at = atomicAdd(&count, __popcll(reach));
+            at = __shfl(at, 0, 64) + __popcll(reach & ((1ull << lane) - 1));
+            if (c.score >= least && at < kMergeCap) list[at] = c;
+        }
+    }
+    __syncthreads();
+    const int n = count;
+    const size_t o = (size_t)blockIdx.x * a.n_out;
+    auto write = [&](int rank, const Cand& c) {
+        const bool none = c.score == 0;
+        a.token[o + rank] = none ? -1 : 0x3ffffff - (int)(c.tie & 0x3ffffff);
+        a.parent[o + rank] = none ? -1 : 63 - (int)(c.tie >> 58);
+        a.score[o + rank] = none ? -INFINITY : (float)unordered64(c.score);
+    };
+    if (n <= kMergeCap) {
+        for (int i = t; i < n; i += kMergeThreads) {
+            const Cand c = list[i];
+            int rank = 0;
+            for (int j = 0; j < n; j++) rank += better(list[j], c);
+            if (rank < a.n_out) write(rank, c);
+        }
+        if (t >= n && t < a.n_out) write(t, Cand{0, 0});
+        return;
+    }
+    Cand acc = {0, 0};
+    for (int l = wave; l < lists; l += NW) {
+        Cand c = {0, 0};
+        if (lane < a.n_out) c = cand_of(l, keys[(size_t)l * a.n_out + lane], lane);
         acc = l == wave ? c : merge64(acc, c);
     }
-    for (int n = NW / 2; n > 0; n >>= 1) {
-        if (wave >= n && wave < 2 * n) half[wave - n][lane] = acc;
+    for (int w = NW / 2; w > 0; w >>= 1) {
+        if (wave >= w && wave < 2 * w) half[wave - w][lane] = acc;
         __syncthreads();
-        if (wave < n) acc = merge64(acc, half[wave][lane]);
+        if (wave < w) acc = merge64(acc, half[wave][lane]);
         __syncthreads();
     }
-    if (wave == 0 && lane < a.n_out) {
-        const size_t o = (size_t)blockIdx.x * a.n_out + lane;
-        const bool none = acc.score == 0;
-        a.token[o] = none ? -1 : 0x3ffffff - (int)(acc.tie & 0x3ffffff);
-        a.parent[o] = none ? -1 : 63 - (int)(acc.tie >> 58);
-        a.score[o] = none ? -INFINITY : (float)unordered64(acc.score);
-    }
+    if (wave == 0 && lane < a.n_out) write(lane, acc);
 }
 
 constexpr int kPartThreads = 256;
-constexpr int kChunk = kPartThreads * 4 * 2;
+
+// Float4s a thread: chunks of 2048 logits where few rows leave CUs idle, of 4096 or 8192
+// (fewer lists to merge) from some 2 workgroups a CU up.
+int beam_v4(const BeamArgs& a) {
+    const long all = (long)a.n_seq * a.n_beams * a.n_vocab;
+    return all >= 512L * 8192 ? 8 : all >= 512L * 4096 ? 4 : 2;
+}
+int beam_chunks(const BeamArgs& a) {
+    const int chunk = kPartThreads * 4 * beam_v4(a);
+    return (a.n_vocab + chunk - 1) / chunk;
+}
 
 }  // namespace
-
-static int beam_chunks(const BeamArgs& a) { return (a.n_vocab + kChunk - 1) / kChunk; }
 
 size_t beam_scratch(const BeamArgs& a) {
     const size_t lists = (size_t)a.n_seq * a.n_beams * beam_chunks(a);
@@ -339,9 +435,16 @@ hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st) {
     for (long r = 0; r < rows; r += 65535) {
         const unsigned n = (unsigned)(rows - r < 65535 ? rows - r : 65535);
         const size_t at = (size_t)r * chunks;
-        k_beam_part<kPartThreads, 2><<<dim3(chunks, n), kPartThreads, 0, st>>>(
-            a.logits + (size_t)r * a.ld, a.ld, a.n_vocab, a.n_out, vec, keys + at * a.n_out, ms + at,
-            ss + at);
+        auto go = [&](auto kernel) {
+            kernel<<<dim3(chunks, n), kPartThreads, 0, st>>>(a.logits + (size_t)r * a.ld, a.ld,
+                                                             a.n_vocab, a.n_out, vec,
+                                                             keys + at * a.n_out, ms + at, ss + at);
+        };
+        switch (beam_v4(a)) {
+            case 8: go(k_beam_part<kPartThreads, 8>); break;
+            case 4: go(k_beam_part<kPartThreads, 4>); break;
+            default: go(k_beam_part<kPartThreads, 2>);
+        }
     }
     k_beam_merge<<<a.n_seq, kMergeThreads, 0, st>>>(a, chunks, keys, ms, ss);
     return hipGetLastError();

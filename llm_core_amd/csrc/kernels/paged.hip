@@ -309,6 +309,11 @@ __device__ __forceinline__ int share_of(long total, long u, int n) {
     return (int)(((u + 1) * n - 1) / total);
 }
 
+__device__ __forceinline__ long uniform(long x) {
+    return (long)(((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(x >> 32)) << 32) |
+                  (uint32_t)__builtin_amdgcn_readfirstlane((int)x));
+}
+
 // One part's stretch of keys in a share.
 struct Span {
     int s, held, tok, j0, j1;
@@ -320,16 +325,16 @@ struct Span {
 // The stretch at unit lo of a share that ends at hi; moves lo behind it.
 __device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, int tile_rows, int unit,
                                           int share, int& s, long& lo, long hi) {
-    while (lo >= cum[s + 1]) s++;
+    while (lo >= uniform(cum[s + 1])) s++;
     Span p;
-    p.s = __builtin_amdgcn_readfirstlane(s);
+    p.s = s;
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, p.s, a.table_ld, a.page_shift);
     const SeqWork w = seq_work(n, a.n_heads / a.n_kv_heads, tile_rows, unit);
     p.held = n.held;
     p.tok = n.tok;
     p.rows = w.rows;
     p.table = a.table + (long)p.s * a.table_ld;
-    const long at = lo - cum[p.s], part = at / w.units, u0 = at - part * w.units;
+    const long at = lo - uniform(cum[p.s]), part = at / w.units, u0 = at - part * w.units;
     const long u1 = min(w.units, u0 + hi - lo);
     p.kvh = __builtin_amdgcn_readfirstlane((int)(part / w.tiles));
     p.tile = __builtin_amdgcn_readfirstlane((int)(part % w.tiles));
@@ -510,7 +515,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     make_plan(a, 16, kFewUnit, cum, scan);
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s <= a.n_seq; s += 256) a.plan[s] = cum[s];
-    const long all = cum[a.n_seq];
+    const long all = uniform(cum[a.n_seq]);
     const int share = share_id();
     const int used = shares_used(a, all);
     if (share >= used) return;
@@ -720,8 +725,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     // take K and the others V.
     constexpr bool kHalves = HD == 64 && NW == 8;
     constexpr int EK = kHalves ? 1 : 4 * HD / (64 * NW), EV = kHalves ? 1 : HD / 64 * 4 / NW;
-    __shared__ uint4 kl[NB][2 * NC * KP * 64];
-    __shared__ uint4 vl[NB][ND * KP * 64];
+    constexpr int VL = 2 * NC * KP * 64;  // V's fragments behind K's
+    __shared__ uint4 frag[NB][VL + ND * KP * 64];
+    __shared__ uint64_t masks[TR];
     __shared__ uint32_t holes[NB];  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
     __shared__ long cum[kPlanSeqs + 1], scan[4];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
@@ -729,7 +735,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     make_plan(a, TR, kManyUnit, cum, scan);
     if (blockIdx.x == 0)
         for (int s = t; s <= a.n_seq; s += 64 * NW) a.plan[s] = cum[s];
-    const long all = cum[a.n_seq];
+    const long all = uniform(cum[a.n_seq]);
     const int share = share_id();
     const int used = shares_used(a, all);
     if (share >= used) return;
@@ -767,17 +773,16 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; e++)
             vrow[e] = __builtin_amdgcn_readlane(krow[e >> 2], 4 * vg + (e & 3));
+        // K: an address a lane; V: a scalar address a row and the lane's offset
         const T* kb = static_cast<const T*>(a.k) + kvh * HD;
-        const T* vb = static_cast<const T*>(a.v) + kvh * HD + vd;
+        const T* vb = static_cast<const T*>(a.v) + kvh * HD;
         if (do_k) {
 #pragma unroll
             for (int p = 0; p < EK; p++) {
                 int tt, j;
                 k_unit(p, tt, j);
-                __builtin_memcpy(
-                    kr[p],
-                    __builtin_assume_aligned(kb + (long)max(tt ? krow[1] : krow[0], 0) * ld + 8 * j, 16),
-                    8 * sizeof(T));
+                const size_t at = (size_t)max(tt ? krow[1] : krow[0], 0) * (size_t)ld + 8 * j;
+                __builtin_memcpy(kr[p], __builtin_assume_aligned(kb + at, 16), 8 * sizeof(T));
             }
         }
         bad_next = 0;
@@ -785,10 +790,11 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
         for (int e = 0; e < 8; e++) bad_next |= (uint32_t)(vrow[e] < 0) << e;
         if (do_v) {
 #pragma unroll
-            for (int e = 0; e < 8; e++)
-                __builtin_memcpy(
-                    vr[e], __builtin_assume_aligned(vb + (long)max(vrow[e], 0) * ld, EV * sizeof(T)),
-                    EV * sizeof(T));
+            for (int e = 0; e < 8; e++) {
+                const T* row = vb + (size_t)max(vrow[e], 0) * (size_t)ld;
+                __builtin_memcpy(vr[e], __builtin_assume_aligned(row + (uint32_t)vd, EV * sizeof(T)),
+                                 EV * sizeof(T));
+            }
         }
     };
     auto put = [&](int buf) {  // split what was fetched into LDS
@@ -804,7 +810,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
                     Parts<T>::split_kv(kr[p], f);
 #pragma unroll
                 for (int q = 0; q < KP; q++)
-                    kl[buf][((tt * NC + j / 4) * KP + q) * 64 + (j & 3) * 16 + n] = f[q];
+                    frag[buf][((tt * NC + j / 4) * KP + q) * 64 + (j & 3) * 16 + n] = f[q];
             }
         }
         if (do_v) {
@@ -821,7 +827,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
                     Parts<T>::split_kv(w, f);
 #pragma unroll
                 for (int q = 0; q < KP; q++)
-                    vl[buf][((d >> 4) * KP + q) * 64 + vg * 16 + (d & 15)] = f[q];
+                    frag[buf][VL + ((d >> 4) * KP + q) * 64 + vg * 16 + (d & 15)] = f[q];
             }
         }
         if (lane == 0 && wave < 4) reinterpret_cast<uint8_t*>(&holes[buf])[wave] = (uint8_t)bad_next;
@@ -831,16 +837,19 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     fetch(sp.j0);
     pages_of(sp.j0 + kStep);
 
+    for (int r = t; r < TR; r += 64 * NW) {
+        const int i = (row0 + r) / G;
+        masks[r] = row0 + r < rows ? seen_mask(a, (long)sp.s * a.max_tok + i, i) : 0;
+    }
     uint4 qf[MW][NC][QP];
     float scale[MW], m[MW], l[MW];
-    bool act[MW], live[MW];
+    bool act[MW];
     f32x4 o[MW][ND];
 #pragma unroll
     for (int w = 0; w < MW; w++) {
         const int rho = row0 + (wave + NW * w) * 16 + n;
         act[w] = row0 + (wave + NW * w) * 16 < rows;
-        live[w] = rho < rows;
-        load_q<HD, T>(a, sp, rho, live[w], qf[w], scale[w]);
+        load_q<HD, T>(a, sp, rho, rho < rows, qf[w], scale[w]);
         m[w] = -INFINITY;
         l[w] = 0.f;
 #pragma unroll
@@ -864,25 +873,31 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
                 for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                     for (int e = 0; e < SUMS; e++) st[w][tt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
+            // fragments are read one product ahead of their use, and no further (the
+            // scheduling barriers: more of them in flight would not fit in registers)
+            uint4 f[2][NA][KP];
+            auto read_k = [&](int i) {  // product i: chunk i / (2 / NA), key tiles from i % (2 / NA) * NA
 #pragma unroll
-            for (int c = 0; c < NC; c++) {
+                for (int x = 0; x < NA; x++)
+#pragma unroll
+                    for (int p = 0; p < KP; p++)
+                        f[i & 1][x][p] =
+                            frag[buf][(((i % (2 / NA) * NA + x) * NC + i / (2 / NA)) * KP + p) * 64 + lane];
+            };
+            read_k(0);
+#pragma unroll
+            for (int i = 0; i < 2 * NC / NA; i++) {
+                if (i + 1 < 2 * NC / NA) read_k(i + 1);
                 const uint4* q[M];
+                f32x4* to[NA][M];
 #pragma unroll
-                for (int w = 0; w < M; w++) q[w] = qf[w][c];
+                for (int w = 0; w < M; w++) {
+                    q[w] = qf[w][i / (2 / NA)];
 #pragma unroll
-                for (int tt = 0; tt < 2; tt += NA) {
-                    uint4 f[NA][KP];
-                    f32x4* to[NA][M];
-#pragma unroll
-                    for (int i = 0; i < NA; i++) {
-#pragma unroll
-                        for (int p = 0; p < KP; p++)
-                            f[i][p] = kl[buf][(((tt + i) * NC + c) * KP + p) * 64 + lane];
-#pragma unroll
-                        for (int w = 0; w < M; w++) to[i][w] = st[w][tt + i];
-                    }
-                    Parts<T>::template scores<NA, M>(f, q, to);
+                    for (int x = 0; x < NA; x++) to[x][w] = st[w][i % (2 / NA) * NA + x];
                 }
+                Parts<T>::template scores<NA, M>(f[i & 1], q, to);
+                __builtin_amdgcn_sched_barrier(0);
             }
             const uint32_t hole = holes[buf], bad = (hole >> (8 * g)) & 255;
             uint4 pf[M][QP];
@@ -891,11 +906,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
             for (int w = 0; w < M; w++) {
                 float keep;
                 const bool masked = hole || jb + kStep > min(sp.held, sp.j1);
-                uint64_t mask = 0;  // wanted in few steps: not kept
-                if (masked && live[w]) {
-                    const int i = (row0 + (wave + NW * w) * 16 + n) / G;
-                    mask = seen_mask(a, (long)sp.s * a.max_tok + i, i);
-                }
+                const uint64_t mask = masked ? masks[(wave + NW * w) * 16 + n] : 0;
                 weights<T>(st[w], scale[w], masked, mask, jb, sp, bad, m[w], l[w], keep, pf[w]);
                 p[w] = pf[w];
                 if (__any(keep != 1.f)) {  // seldom after the first steps
@@ -903,18 +914,25 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
                     for (int d = 0; d < ND; d++) o[w][d] *= keep;
                 }
             }
+            auto read_v = [&](int i) {
 #pragma unroll
-            for (int d = 0; d < ND; d += NA) {
-                uint4 f[NA][KP];
+                for (int x = 0; x < NA; x++)
+#pragma unroll
+                    for (int q = 0; q < KP; q++)
+                        f[i & 1][x][q] = frag[buf][VL + ((i * NA + x) * KP + q) * 64 + lane];
+            };
+            __builtin_amdgcn_sched_barrier(0);
+            read_v(0);
+#pragma unroll
+            for (int i = 0; i < ND / NA; i++) {
+                if (i + 1 < ND / NA) read_v(i + 1);
                 f32x4* to[NA][M];
 #pragma unroll
-                for (int i = 0; i < NA; i++) {
+                for (int x = 0; x < NA; x++)
 #pragma unroll
-                    for (int q = 0; q < KP; q++) f[i][q] = vl[buf][((d + i) * KP + q) * 64 + lane];
-#pragma unroll
-                    for (int w = 0; w < M; w++) to[i][w] = &o[w][d + i];
-                }
-                Parts<T>::template product<NA, M>(f, p, to);
+                    for (int w = 0; w < M; w++) to[x][w] = &o[w][i * NA + x];
+                Parts<T>::template product<NA, M>(f[i & 1], p, to);
+                __builtin_amdgcn_sched_barrier(0);
             }
         };
         if (MW == 2 && act[MW - 1])
@@ -938,7 +956,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
         if (!act[w]) continue;
         l[w] = rows_sum(l[w]);
         const int in = (wave + NW * w) * 16;  // the tile's first row within the workgroup's
-        if (!live[w]) continue;
+        if (row0 + in + n >= rows) continue;
         float* dst = whole ? a.out + out_row(a, sp, row0 + in + n) * HD
                            : a.part + ((long)sp.slot * TR + in + n) * HD;
         if (!whole && g == 0) a.part_ml[sp.slot * TR + in + n] = make_float2(m[w], l[w]);
@@ -1327,16 +1345,20 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
 }
 
 // Query rows of a KV head that a workgroup takes: the fewest that hold them all, so that
-// the cache is read once; with 256 elements a head 256 rows' sums do not fit.
-int tile_rows(int rows, int head_dim) {
+// the cache is read once, as far as two tiles' operands and sums fit in a wave's 256
+// registers: at 64 elements a head, and at 128 with F16 pages' two parts of q.  (F32 at
+// 128: 40 registers spilt, 16 trees of 48 tokens @8191 in 446 us against 402 with
+// 128-row tiles that read the cache twice.)
+int tile_rows(int rows, int head_dim, int kv_type) {
     if (rows <= 16) return 16;
     if (rows <= 64) return 64;
-    return rows <= 128 || head_dim == 256 ? 128 : 256;
+    return rows > 128 && (head_dim == 64 || (head_dim == 128 && kv_type == AXF_TYPE_F16)) ? 256 : 128;
 }
 
 template <int HD, class T>
 hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), HD);
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), HD,
+                             sizeof(T) == 2 ? AXF_TYPE_F16 : AXF_TYPE_F32);
     if (tr == 16) {
         k_attn_paged_few<HD, T><<<a.shares, 64 * kFewWaves, 0, st>>>(a);
     } else if (tr == 64) {
@@ -1344,7 +1366,8 @@ hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
     } else if (tr == 128) {
         k_attn_paged_many<HD, T, 8, 1><<<a.shares, 512, 0, st>>>(a);
     } else {
-        if constexpr (HD < 256) k_attn_paged_many<HD, T, 8, 2><<<a.shares, 512, 0, st>>>(a);
+        if constexpr (HD == 64 || (HD == 128 && sizeof(T) == 2))
+            k_attn_paged_many<HD, T, 8, 2><<<a.shares, 512, 0, st>>>(a);
     }
     const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
     k_attn_paged_join<HD, T><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(
@@ -1374,10 +1397,10 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 
 // Workgroups of the launch: as many as run at once (two of 4 waves a CU, one of 8), or as
 // few as have a unit each by the caller's estimate of the lengths.
-void attn_paged_plan(PagedArgs& a, int head_dim, int max_len) {
+void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
-    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, head_dim);
+    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, head_dim, kv_type);
     const long seqs = a.n_seq < kPlanSeqs ? a.n_seq : kPlanSeqs;
     const long units = (longest + (tr == 16 ? kFewUnit : kManyUnit) - 1) /
                        (tr == 16 ? kFewUnit : kManyUnit) * seqs * a.n_kv_heads * ((rows + tr - 1) / tr);
@@ -1386,14 +1409,14 @@ void attn_paged_plan(PagedArgs& a, int head_dim, int max_len) {
     a.shares = (int)((shares + 7) & ~7L);
 }
 
-size_t attn_paged_scratch(const PagedArgs& a, int head_dim) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim);
+size_t attn_paged_scratch(const PagedArgs& a, int kv_type, int head_dim) {
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim, kv_type);
     return (kPlanSeqs + 1) * sizeof(long) + (size_t)2 * a.shares * tr * (head_dim + 2) * 4 + 16;
 }
 
 hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, void* scratch,
                              hipStream_t st) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim);
+    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim, kv_type);
     for (int s = 0; s < a.n_seq; s += kPlanSeqs) {
         PagedArgs b = a;
         const long row = (long)s * a.max_tok;
