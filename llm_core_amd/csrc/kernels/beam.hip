@@ -35,26 +35,25 @@ __device__ __forceinline__ double unordered64(uint64_t o) {
     return __longlong_as_double((int64_t)((o >> 63) ? (o ^ 0x8000000000000000ull) : ~o));
 }
 
-// exp(x) for x <= 0 to 2e-13 of its value: 2^k times the Taylor polynomial of
-// degree 10 on [-ln2/2, ln2/2] (its first term left out: 0.347^11 / 11! = 2.2e-13).
-// Below -708 zero; NaN stays NaN.
-__device__ __forceinline__ double exp_neg(double x) {
-    const double k = __builtin_rint(x * 1.4426950408889634074);
-    double r = __builtin_fma(k, -6.93147180369123816490e-01, x);  // ln 2 in two parts
-    r = __builtin_fma(k, -1.90821492927058770002e-10, r);
-    double p = 1.0 / 3628800;
-    p = __builtin_fma(p, r, 1.0 / 362880);
-    p = __builtin_fma(p, r, 1.0 / 40320);
-    p = __builtin_fma(p, r, 1.0 / 5040);
-    p = __builtin_fma(p, r, 1.0 / 720);
-    p = __builtin_fma(p, r, 1.0 / 120);
-    p = __builtin_fma(p, r, 1.0 / 24);
+// 2^(j / 32), j < 32, in LDS: exp_neg's table.
+__device__ __forceinline__ void fill_exp_table(double* tab) {
+    if (threadIdx.x < 32) tab[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32));
+}
+
+// exp(x) for x <= 0 to 2e-12 of its value: 2^(k / 32) from the table times the Taylor
+// polynomial of degree 4 on [-ln2/64, ln2/64] (its first term left out: 0.01083^5 / 5! =
+// 1.2e-12).  Below -708 zero; NaN stays NaN.
+__device__ __forceinline__ double exp_neg(double x, const double* tab) {
+    const double k = __builtin_rint(x * (32 * 1.4426950408889634074));
+    // ln 2 / 32 in one part: k < 33000 leaves its last bit's error below 2e-14
+    const double r = __builtin_fma(k, -6.93147180559945309417e-01 / 32, x);
+    double p = 1.0 / 24;
     p = __builtin_fma(p, r, 1.0 / 6);
     p = __builtin_fma(p, r, 0.5);
     p = __builtin_fma(p, r, 1.0);
-    p = __builtin_fma(p, r, 1.0);
-    const int e = (int)fmax(k, -1022.0);
-    const double y = __builtin_ldexp(p, e);
+    const int n = (int)fmax(k, -32768.0);
+    const double t = tab[n & 31];
+    const double y = __builtin_ldexp(__builtin_fma(p * r, t, t), n >> 5);
     return x < -708.0 ? 0.0 : y;
 }
 
@@ -64,153 +63,92 @@ __device__ __forceinline__ double wave_sum64(double v) {
     return v;
 }
 
-// The k-th largest of the wave's 64 keys (k >= 1; keys differ unless 0): bit by
-// bit from the top, the largest value that at least k keys reach.
-__device__ __forceinline__ uint64_t kth_of_wave(uint64_t key, int k) {
-    const uint32_t hi = (uint32_t)(key >> 32), lo = (uint32_t)key;
+// The k-th largest of the wave's 64 values (k >= 1): bit by bit from the top, the
+// largest value that at least k of them reach.
+__device__ __forceinline__ uint32_t kth_of_wave(uint32_t v, int k) {
     uint32_t t = 0;
     for (int b = 31; b >= 0; b--) {
         const uint32_t c = t | (1u << b);
-        if (__popcll(__ballot(hi >= c)) >= k) t = c;
+        if (__popcll(__ballot(v >= c)) >= k) t = c;
     }
-    const int above = __popcll(__ballot(hi > t));
-    const bool same = hi == t;
-    if (__popcll(__ballot(same)) == k - above) {  // all of the equal ones: their least
-        uint32_t u = same ? lo : 0xffffffffu;
-#pragma unroll
-        for (int off = 32; off > 0; off >>= 1) u = min(u, (uint32_t)__shfl_xor((int)u, off, 64));
-        return ((uint64_t)t << 32) | u;
-    }
-    uint32_t v = 0;
-    for (int b = 31; b >= 0; b--) {
-        const uint32_t c = v | (1u << b);
-        if (__popcll(__ballot(same && lo >= c)) >= k - above) v = c;
-    }
-    return ((uint64_t)t << 32) | v;
+    return t;
 }
 
 constexpr int kCap = 512;  // keys ranked at once
 
 // Chunk blockIdx.x of row blockIdx.y: keys[n_out] (largest first, 0: none), m, s.
 // Thread t holds elements 4 (t + NT j) .. +3, j < V4, of the chunk: the same ones
-// whatever the row's alignment.  Every thread's largest key is known without a
-// sort; the n_out-th largest of a wave's 64 is a bound that n_out keys reach, and
-// the keys that reach the largest such bound (some n_out to 3 n_out of them) are
-// ranked by counting.
+// whatever the row's alignment.  Every thread's largest logit is known without a
+// sort; the n_out-th largest of a wave's 64 is a bound that n_out logits reach, and
+// the logits that reach the largest such bound (some n_out to 3 n_out of them) are
+// ranked by counting.  Where equal or unevenly spread logits leave too many, the
+// n_out-th largest key of all is found bit by bit.
 template <int NT, int V4>
 __global__ __launch_bounds__(NT) void k_beam_part(const float* __restrict__ logits, int ld, int n_vocab,
                                                   int n_out, int vec, uint64_t* __restrict__ keys,
                                                   float* __restrict__ ms, double* __restrict__ ss) {
     constexpr int NW = NT / 64, CH = NT * V4 * 4;
     __shared__ uint64_t list[kCap];
-    __shared__ uint64_t bound[NW];
+    __shared__ double tab[32], wsum[NW];
+    __shared__ uint32_t bound[NW];
     __shared__ float wm[NW];
-    __shared__ double wsum[NW];
     __shared__ int count;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const float* x = logits + (size_t)blockIdx.y * ld;
     const int base = blockIdx.x * CH;
     float v[V4 * 4];
+    if (vec && base + CH <= n_vocab) {
 #pragma unroll
-    for (int j = 0; j < V4; j++) {
-        const int i = base + 4 * (t + NT * j);
-        if (vec && i + 3 < n_vocab) {
-            const float4 f = *reinterpret_cast<const float4*>(x + i);
+        for (int j = 0; j < V4; j++) {
+            const float4 f = *reinterpret_cast<const float4*>(x + base + 4 * (t + NT * j));
             v[4 * j] = f.x;
             v[4 * j + 1] = f.y;
             v[4 * j + 2] = f.z;
             v[4 * j + 3] = f.w;
-        } else {
+        }
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; e++) v[4 * j + e] = i + e < n_vocab ? x[i + e] : -INFINITY;
+        for (int j = 0; j < V4 * 4; j++) {
+            const int i = base + 4 * (t + NT * (j >> 2)) + (j & 3);
+            v[j] = i < n_vocab ? x[i] : -INFINITY;
         }
     }
-    auto key_of = [&](int j, int e) {
-        const int i = base + 4 * (t + NT * j) + e;
-        return i < n_vocab ? ((uint64_t)ordered32(v[4 * j + e]) << 32) | (uint32_t)~i : 0ull;
-    };
-    uint64_t best = 0;
-    float m = -INFINITY;
+    fill_exp_table(tab);
+    float m = v[0];
 #pragma unroll
-    for (int j = 0; j < V4; j++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint64_t k = key_of(j, e);
-            best = k > best ? k : best;
-            m = fmaxf(m, v[4 * j + e]);
-        }
-    }
+    for (int j = 1; j < V4 * 4; j++) m = fmaxf(m, v[j]);
+    const uint32_t mine = kth_of_wave(ordered32(m), n_out);
     m = wave_max(m);
-    const uint64_t mine = kth_of_wave(best, n_out);
     if (lane == 0) {
         bound[wave] = mine;
         wm[wave] = m;
     }
     if (t == 0) count = 0;
     __syncthreads();
-    uint64_t least = bound[0];
+    // -inf is no continuation's logit
+    uint32_t at_least = ordered32(-__FLT_MAX__);
     m = wm[0];
 #pragma unroll
-    for (int w = 1; w < NW; w++) {
-        least = bound[w] > least ? bound[w] : least;
+    for (int w = 0; w < NW; w++) {
+        at_least = max(at_least, bound[w]);
         m = fmaxf(m, wm[w]);
     }
-    least = least ? least : 1;  // 0: no element
-    // the keys that reach the bound
-    int reach = 0;
+    const float least = unordered32(at_least);
+    uint32_t hits = 0;
 #pragma unroll
-    for (int j = 0; j < V4; j++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) reach += key_of(j, e) >= least;
-    const int at = reach ? atomicAdd(&count, reach) : 0;
-    __syncthreads();
-    int n = count;
-    if (n > kCap) {
-        // few threads hold many large keys: the n_out-th largest of all, bit by bit
-        uint64_t c = 0;
-        for (int b = 63; b >= 0; b--) {
-            const uint64_t probe = c | (1ull << b);
-            int r = 0;
-#pragma unroll
-            for (int j = 0; j < V4; j++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) r += key_of(j, e) >= probe;
-            __syncthreads();
-            if (t == 0) count = 0;
-            __syncthreads();
-            if (r) atomicAdd(&count, r);
-            __syncthreads();
-            if (count >= n_out) c = probe;
-        }
-        least = c ? c : 1;
-        reach = 0;
-#pragma unroll
-        for (int j = 0; j < V4; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) reach += key_of(j, e) >= least;
-        __syncthreads();
-        if (t == 0) count = 0;
-        __syncthreads();
-        int o = reach ? atomicAdd(&count, reach) : 0;
-        if (reach)
-            for (int j = 0; j < V4; j++)
-                for (int e = 0; e < 4; e++)
-                    if (key_of(j, e) >= least) list[o++] = key_of(j, e);
-        __syncthreads();
-        n = count;
-    } else if (reach) {
-        int o = at;
-#pragma unroll
-        for (int j = 0; j < V4; j++)
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                if (key_of(j, e) >= least) list[o++] = key_of(j, e);
+    for (int j = 0; j < V4 * 4; j++) hits |= v[j] >= least ? 1u << j : 0;
+    auto index_of = [&](int j) { return base + 4 * (t + NT * (j >> 2)) + (j & 3); };
+    auto key_of = [&](int i, float y) { return ((uint64_t)ordered32(y) << 32) | (uint32_t)~i; };
+    // few: read again rather than picked from registers by a variable
+    for (uint32_t h = hits; h; h &= h - 1) {
+        const int i = index_of(__builtin_ctz(h)), at = atomicAdd(&count, 1);
+        if (at < kCap) list[at] = key_of(i, x[i]);
     }
     // sum of exponentials; a NaN or +inf logit makes it NaN, as it does the row's
     const double top = m == -INFINITY ? 0.0 : (double)m;
     double s = 0.0;
 #pragma unroll
-    for (int j = 0; j < V4 * 4; j++) s += exp_neg((double)v[j] - top);
+    for (int j = 0; j < V4 * 4; j++) s += exp_neg((double)v[j] - top, tab);
     s = wave_sum64(s);
     if (lane == 0) wsum[wave] = s;
     __syncthreads();
@@ -221,6 +159,32 @@ __global__ __launch_bounds__(NT) void k_beam_part(const float* __restrict__ logi
         for (int w = 1; w < NW; w++) sum += wsum[w];
         ss[chunk] = sum;
         ms[chunk] = m;
+    }
+    int n = count;
+    if (n > kCap) {
+        uint64_t c = 0;
+        for (int b = 63; b >= 0; b--) {
+            const uint64_t probe = c | (1ull << b);
+            int r = 0;
+#pragma unroll
+            for (int j = 0; j < V4 * 4; j++) r += v[j] >= least && key_of(index_of(j), v[j]) >= probe;
+            __syncthreads();
+            if (t == 0) count = 0;
+            __syncthreads();
+            if (r) atomicAdd(&count, r);
+            __syncthreads();
+            if (count >= n_out) c = probe;
+        }
+        __syncthreads();
+        if (t == 0) count = 0;
+        __syncthreads();
+        for (uint32_t h = hits; h; h &= h - 1) {
+            const int i = index_of(__builtin_ctz(h));
+            const uint64_t k = key_of(i, x[i]);
+            if (k >= c) list[atomicAdd(&count, 1)] = k;  // keys differ: n_out of them
+        }
+        __syncthreads();
+        n = count;
     }
     uint64_t* out = keys + chunk * n_out;
     for (int c = t; c < n; c += NT) {
@@ -261,12 +225,7 @@ __device__ __forceinline__ Cand merge64(Cand a, Cand b) {
 
 // The k-th largest score of the wave's 64 (scores may be equal), or 0 with fewer.
 __device__ __forceinline__ uint64_t kth_score(uint64_t s, int k) {
-    const uint32_t hi = (uint32_t)(s >> 32), lo = (uint32_t)s;
-    uint32_t t = 0;
-    for (int b = 31; b >= 0; b--) {
-        const uint32_t c = t | (1u << b);
-        if (__popcll(__ballot(hi >= c)) >= k) t = c;
-    }
+    const uint32_t hi = (uint32_t)(s >> 32), lo = (uint32_t)s, t = kth_of_wave(hi, k);
     const int above = __popcll(__ballot(hi > t));
     const bool same = hi == t;
     uint32_t v = 0;
@@ -277,7 +236,8 @@ __device__ __forceinline__ uint64_t kth_score(uint64_t s, int k) {
     return ((uint64_t)t << 32) | v;
 }
 
-constexpr int kMergeCap = 512;  // candidates ranked at once
+constexpr int kMergeCap = 512;    // candidates ranked at once
+constexpr int kMergePicks = 512;  // lists looked into
 
 // The chunks' lists of one sequence.  Their heads come first: a score that n_out heads
 // reach bounds what can be among the n_out best, which leaves few lists and few of
@@ -292,19 +252,23 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
     __shared__ int over[64];
     __shared__ Cand half[NW / 2][64];
     __shared__ Cand list[kMergeCap];
+    __shared__ double tab[32];
     __shared__ uint64_t bound[NW];
-    __shared__ int count;
+    __shared__ int picks[kMergePicks];
+    __shared__ int count, picked;
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const size_t row0 = (size_t)blockIdx.x * a.n_beams;
     const int lists = a.n_beams * chunks;
     keys += row0 * chunks * a.n_out;
-    if (t == 0) count = 0;
+    if (t == 0) count = picked = 0;
+    fill_exp_table(tab);
     if (t < a.n_beams) {
         cums[t] = (double)a.cum[row0 + t];
         over[t] = a.done && a.done[row0 + t] != 0;
     }
     // the first round's heads are in flight while the sums are joined
     const uint64_t head0 = t < lists ? keys[(size_t)t * a.n_out] : 0;
+    __syncthreads();
     for (int b = wave; b < a.n_beams; b += NW) {
         const float* mr = ms + (row0 + b) * chunks;
         const double* sr = ss + (row0 + b) * chunks;
@@ -318,8 +282,8 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
         for (int c = lane + 64; c < chunks; c += 64) m = fmaxf(m, mr[c]);
         m = wave_max(m);
         const double top = m == -INFINITY ? 0.0 : (double)m;
-        s = s0 * exp_neg((double)m0 - top);
-        for (int c = lane + 64; c < chunks; c += 64) s += sr[c] * exp_neg((double)mr[c] - top);
+        s = s0 * exp_neg((double)m0 - top, tab);
+        for (int c = lane + 64; c < chunks; c += 64) s += sr[c] * exp_neg((double)mr[c] - top, tab);
         s = wave_sum64(s);
         // all logits -inf: log 0, and every score -inf - -inf
         if (lane == 0) lse[b] = top + log(s);
@@ -353,24 +317,25 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
     uint64_t least = 1;
 #pragma unroll
     for (int w = 0; w < NW; w++) least = bound[w] > least ? bound[w] : least;
-    // the lists whose head reaches it, a wave's lanes over one list's entries
-    for (int l0 = wave * 64; l0 < lists; l0 += kMergeThreads) {
-        const int l = l0 + lane;
-        const bool in = l < lists &&
-                        cand_of(l, l == t ? head0 : keys[(size_t)l * a.n_out], 0).score >= least;
-        for (uint64_t left = __ballot(in); left; left &= left - 1) {
-            const int pick = l0 + __builtin_ctzll(left);
-            Cand c = {0, 0};
-            if (lane < a.n_out) c = cand_of(pick, keys[(size_t)pick * a.n_out + lane], lane);
-            const uint64_t reach = __ballot(c.score >= least);
-            int at = 0;
-            if (lane == 0) at = atomicAdd(&count, __popcll(reach));
-            at = __shfl(at, 0, 64) + __popcll(reach & ((1ull << lane) - 1));
-            if (c.score >= least && at < kMergeCap) list[at] = c;
+    // the lists whose head reaches it, dealt out to the waves, a lane an entry
+    for (int l = t; l < lists; l += kMergeThreads)
+        if (cand_of(l, l == t ? head0 : keys[(size_t)l * a.n_out], 0).score >= least) {
+            const int at = atomicAdd(&picked, 1);
+            if (at < kMergePicks) picks[at] = l;
         }
+    __syncthreads();
+    const int np = picked;
+    for (int i = wave; i < min(np, kMergePicks); i += NW) {
+        Cand c = {0, 0};
+        if (lane < a.n_out) c = cand_of(picks[i], keys[(size_t)picks[i] * a.n_out + lane], lane);
+        const uint64_t reach = __ballot(c.score >= least);
+        int at = 0;
+        if (lane == 0) at = atomicAdd(&count, __popcll(reach));
+        at = __shfl(at, 0, 64) + __popcll(reach & ((1ull << lane) - 1));
+        if (c.score >= least && at < kMergeCap) list[at] = c;
     }
     __syncthreads();
-    const int n = count;
+    const int n = np > kMergePicks ? kMergeCap + 1 : count;
     const size_t o = (size_t)blockIdx.x * a.n_out;
     auto write = [&](int rank, const Cand& c) {
         const bool none = c.score == 0;
