@@ -335,7 +335,7 @@ struct PagedArgs {
     const uint64_t* mask;  // nullptr: causal among the tokens
     const int* pos;        // nullptr: q is turned already
     const float *cos_t, *sin_t;
-    int n_pos, n_seq, max_tok, n_heads, n_kv_heads;
+    int n_pos, n_seq, max_tok, n_heads, n_kv_heads, group;  // group: heads a KV head
     int n_pages, page_shift;
     float* out;
     uint8_t* outq8;

@@ -187,6 +187,7 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
     a.max_tok = max_tok;
     a.n_heads = n_heads;
     a.n_kv_heads = kv->n_kv_heads;
+    a.group = n_heads / kv->n_kv_heads;
     a.n_pages = kv->n_pages;
     a.page_shift = page_shift(kv);
     a.out = out;

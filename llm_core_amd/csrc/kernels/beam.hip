@@ -35,9 +35,27 @@ __device__ __forceinline__ double unordered64(uint64_t o) {
     return __longlong_as_double((int64_t)((o >> 63) ? (o ^ 0x8000000000000000ull) : ~o));
 }
 
-// 2^(j / 32), j < 32, in LDS: exp_neg's table.
+// 2^(j / 32), j < 32, to the nearest double: exp_neg's table, copied to LDS.
+__device__ const double kExpTable[32] = {
+    1.0, 1.0218971486541166,
+    1.0442737824274138, 1.0671404006768237,
+    1.0905077326652577, 1.1143867425958924,
+    1.1387886347566916, 1.1637248587775775,
+    1.189207115002721, 1.215247359980469,
+    1.241857812073484, 1.2690509571917332,
+    1.2968395546510096, 1.3252366431597413,
+    1.3542555469368927, 1.383909881963832,
+    1.4142135623730951, 1.4451808069770467,
+    1.4768261459394993, 1.5091644275934228,
+    1.5422108254079407, 1.5759808451078865,
+    1.6104903319492543, 1.645755478153965,
+    1.681792830507429, 1.718619298122478,
+    1.7562521603732995, 1.7947090750031072,
+    1.8340080864093424, 1.8741676341103,
+    1.9152065613971474, 1.9571441241754002,
+};
 __device__ __forceinline__ void fill_exp_table(double* tab) {
-    if (threadIdx.x < 32) tab[threadIdx.x] = exp2(threadIdx.x * (1.0 / 32));
+    if (threadIdx.x < 32) tab[threadIdx.x] = kExpTable[threadIdx.x];
 }
 
 // exp(x) for x <= 0 to 2e-12 of its value: 2^(k / 32) from the table times the Taylor
@@ -96,6 +114,7 @@ __global__ __launch_bounds__(NT) void k_beam_part(const float* __restrict__ logi
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const float* x = logits + (size_t)blockIdx.y * ld;
     const int base = blockIdx.x * CH;
+    fill_exp_table(tab);
     float v[V4 * 4];
     if (vec && base + CH <= n_vocab) {
 #pragma unroll
@@ -113,7 +132,6 @@ __global__ __launch_bounds__(NT) void k_beam_part(const float* __restrict__ logi
             v[j] = i < n_vocab ? x[i] : -INFINITY;
         }
     }
-    fill_exp_table(tab);
     float m = v[0];
 #pragma unroll
     for (int j = 1; j < V4 * 4; j++) m = fmaxf(m, v[j]);
@@ -370,11 +388,11 @@ __global__ __launch_bounds__(kMergeThreads) void k_beam_merge(
 
 constexpr int kPartThreads = 256;
 
-// Float4s a thread: chunks of 2048 logits where few rows leave CUs idle, of 4096 or 8192
-// (fewer lists to merge) from some 2 workgroups a CU up.
+// Float4s a thread: chunks of 2048 logits where few rows leave CUs idle, of 4096 (fewer
+// lists to merge) from two workgroups a CU up.  8 x 8 beams of 151936: 29.0 us, with
+// 2048 31.9, with 8192 (one round of waves, nothing in flight under its arithmetic) 31.4.
 int beam_v4(const BeamArgs& a) {
-    const long all = (long)a.n_seq * a.n_beams * a.n_vocab;
-    return all >= 512L * 8192 ? 8 : all >= 512L * 4096 ? 4 : 2;
+    return (long)a.n_seq * a.n_beams * a.n_vocab >= 512L * 4096 ? 4 : 2;
 }
 int beam_chunks(const BeamArgs& a) {
     const int chunk = kPartThreads * 4 * beam_v4(a);
@@ -405,11 +423,10 @@ hipError_t launch_beam_select(const BeamArgs& a, hipStream_t st) {
                                                              a.n_vocab, a.n_out, vec,
                                                              keys + at * a.n_out, ms + at, ss + at);
         };
-        switch (beam_v4(a)) {
-            case 8: go(k_beam_part<kPartThreads, 8>); break;
-            case 4: go(k_beam_part<kPartThreads, 4>); break;
-            default: go(k_beam_part<kPartThreads, 2>);
-        }
+        if (beam_v4(a) == 4)
+            go(k_beam_part<kPartThreads, 4>);
+        else
+            go(k_beam_part<kPartThreads, 2>);
     }
     k_beam_merge<<<a.n_seq, kMergeThreads, 0, st>>>(a, chunks, keys, ms, ss);
     return hipGetLastError();

@@ -262,15 +262,24 @@ __device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, i
 // k_attn_paged_join adds.
 constexpr int kPlanSeqs = 256;  // sequences a launch
 
+// a / b of whole numbers, a >= 0, b > 0, a / b < 2^51 (no 64-bit integer division in
+// hardware): the rounded quotient is off by one at the most.
+__device__ __forceinline__ long div_whole(long a, long b) {
+    long q = (long)((double)a / (double)b);
+    const long r = a - q * b;
+    return r < 0 ? q - 1 : (r >= b ? q + 1 : q);
+}
+
 struct SeqWork {
     int rows, tiles;
     long units;  // of one part
 };
+// tile_rows and unit are powers of two
 __device__ __forceinline__ SeqWork seq_work(const SeqLen& n, int G, int tile_rows, int unit) {
     SeqWork w;
     w.rows = n.tok * G;
-    w.tiles = (w.rows + tile_rows - 1) / tile_rows;
-    w.units = w.tiles ? ((long)n.held + n.tok + unit - 1) / unit : 0;
+    w.tiles = (w.rows + tile_rows - 1) >> __builtin_ctz(tile_rows);
+    w.units = w.tiles ? ((long)n.held + n.tok + unit - 1) >> __builtin_ctz(unit) : 0;
     return w;
 }
 
@@ -281,7 +290,7 @@ __device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, int
     long w = 0;
     if (t < a.n_seq) {
         const SeqWork k = seq_work(seq_len(a.len, a.n_tok, a.max_tok, t, a.table_ld, a.page_shift),
-                                   a.n_heads / a.n_kv_heads, tile_rows, unit);
+                                   a.group, tile_rows, unit);
         w = k.units * k.tiles * a.n_kv_heads;
     }
 #pragma unroll
@@ -304,9 +313,11 @@ __device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, int
 __device__ __forceinline__ int shares_used(const PagedArgs& a, long total) {
     return (int)min((long)a.shares, total);
 }
-__device__ __forceinline__ long share_start(long total, int w, int n) { return total * w / n; }
+__device__ __forceinline__ long share_start(long total, int w, int n) {
+    return div_whole(total * w, n);
+}
 __device__ __forceinline__ int share_of(long total, long u, int n) {
-    return (int)(((u + 1) * n - 1) / total);
+    return (int)div_whole((u + 1) * n - 1, total);
 }
 
 __device__ __forceinline__ long uniform(long x) {
@@ -329,15 +340,15 @@ __device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, i
     Span p;
     p.s = s;
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, p.s, a.table_ld, a.page_shift);
-    const SeqWork w = seq_work(n, a.n_heads / a.n_kv_heads, tile_rows, unit);
+    const SeqWork w = seq_work(n, a.group, tile_rows, unit);
     p.held = n.held;
     p.tok = n.tok;
     p.rows = w.rows;
     p.table = a.table + (long)p.s * a.table_ld;
-    const long at = lo - uniform(cum[p.s]), part = at / w.units, u0 = at - part * w.units;
-    const long u1 = min(w.units, u0 + hi - lo);
-    p.kvh = __builtin_amdgcn_readfirstlane((int)(part / w.tiles));
-    p.tile = __builtin_amdgcn_readfirstlane((int)(part % w.tiles));
+    const long at = lo - uniform(cum[p.s]), part = uniform(div_whole(at, w.units));
+    const long u0 = at - part * w.units, u1 = min(w.units, u0 + hi - lo);
+    p.kvh = __builtin_amdgcn_readfirstlane((int)((uint32_t)part / (uint32_t)w.tiles));
+    p.tile = (int)part - p.kvh * w.tiles;
     p.j0 = __builtin_amdgcn_readfirstlane((int)(u0 * unit));
     p.j1 = __builtin_amdgcn_readfirstlane((int)min(u1 * unit, (long)n.held + n.tok));
     p.slot = u0 > 0 ? 2 * share : (u1 < w.units ? 2 * share + 1 : -1);
@@ -354,7 +365,7 @@ __device__ __forceinline__ uint64_t seen_mask(const PagedArgs& a, long row, int 
 template <int HD, class T>
 __device__ __forceinline__ void row_careful(const PagedArgs& a, int s, int i, int h, float (&y)[HD / 64]) {
     constexpr int E = HD / 64, U = 4;
-    const int lane = threadIdx.x & 63, kvh = h / (a.n_heads / a.n_kv_heads);
+    const int lane = threadIdx.x & 63, kvh = h / a.group;
     const long row = (long)s * a.max_tok + i, ld = (long)a.n_kv_heads * HD;
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
     const int* table = a.table + (long)s * a.table_ld;
@@ -410,7 +421,7 @@ template <int HD, class T>
 __device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, bool live,
                                        uint4 (&qf)[HD / 32][Parts<T>::QP], float& scale) {
     constexpr int NC = HD / 32;
-    const int g = (threadIdx.x & 63) >> 4, G = a.n_heads / a.n_kv_heads;
+    const int g = (threadIdx.x & 63) >> 4, G = a.group;
     const int i = rho / G, h = sp.kvh * G + rho % G;
     float x[NC][8];
 #pragma unroll
@@ -499,7 +510,7 @@ __device__ __forceinline__ int share_id() {
 
 // Row of out (of HD floats) that query row rho of a span is.
 __device__ __forceinline__ long out_row(const PagedArgs& a, const Span& sp, int rho) {
-    const int G = a.n_heads / a.n_kv_heads;
+    const int G = a.group;
     return ((long)sp.s * a.max_tok + rho / G) * a.n_heads + sp.kvh * G + rho % G;
 }
 
@@ -511,7 +522,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
     __shared__ long cum[kPlanSeqs + 1], scan[4];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
+    const int n = lane & 15, g = lane >> 4, G = a.group;
     make_plan(a, 16, kFewUnit, cum, scan);
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s <= a.n_seq; s += 256) a.plan[s] = cum[s];
@@ -519,8 +530,8 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     const int share = share_id();
     const int used = shares_used(a, all);
     if (share >= used) return;
-    long lo = share_start(all, share, used);
-    const long hi = share_start(all, share + 1, used);
+    long lo = uniform(share_start(all, share, used));
+    const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
     while (lo < hi) {
     const Span sp = next_span(a, cum, 16, kFewUnit, share, seq, lo, hi);
@@ -731,7 +742,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     __shared__ uint32_t holes[NB];  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
     __shared__ long cum[kPlanSeqs + 1], scan[4];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
-    const int n = lane & 15, g = lane >> 4, G = a.n_heads / a.n_kv_heads;
+    const int n = lane & 15, g = lane >> 4, G = a.group;
     make_plan(a, TR, kManyUnit, cum, scan);
     if (blockIdx.x == 0)
         for (int s = t; s <= a.n_seq; s += 64 * NW) a.plan[s] = cum[s];
@@ -739,8 +750,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     const int share = share_id();
     const int used = shares_used(a, all);
     if (share >= used) return;
-    long lo = share_start(all, share, used);
-    const long hi = share_start(all, share + 1, used);
+    long lo = uniform(share_start(all, share, used));
+    const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
     while (lo < hi) {
     const Span sp = next_span(a, cum, TR, kManyUnit, share, seq, lo, hi);
@@ -980,26 +991,28 @@ template <int HD, class T>
 __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows, int unit) {
     constexpr int E = HD / 64, U = 8;
     const int lane = threadIdx.x & 63;
-    const long w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
-    if (w >= (long)a.n_seq * a.max_tok * a.n_heads) return;
-    const int h = (int)(w % a.n_heads), i = (int)(w / a.n_heads % a.max_tok);
-    const int s = (int)(w / a.n_heads / a.max_tok), G = a.n_heads / a.n_kv_heads;
+    const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
+    if (w >= (uint32_t)a.n_seq * a.max_tok * a.n_heads) return;  // at most 2^26
+    const uint32_t token = w / (uint32_t)a.n_heads;
+    const int h = (int)(w - token * a.n_heads), s = (int)(token / (uint32_t)a.max_tok);
+    const int i = (int)token - s * a.max_tok, G = a.group;
     const long all = a.plan[a.n_seq], before = a.plan[s];
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
     if (i >= n.tok) return;
     const SeqWork sw = seq_work(n, G, tile_rows, unit);
-    const int rho = i * G + h % G, tile = rho / tile_rows;
-    const long p0 = before + ((long)(h / G) * sw.tiles + tile) * sw.units;
+    const int kvh = (int)((uint32_t)h / (uint32_t)G), rho = i * G + h - kvh * G;
+    const int tile = rho >> __builtin_ctz(tile_rows);
+    const long p0 = before + ((long)kvh * sw.tiles + tile) * sw.units;
     const int shares = shares_used(a, all);
     const int w1 = __builtin_amdgcn_readfirstlane(share_of(all, p0, shares));
     const int w2 = __builtin_amdgcn_readfirstlane(share_of(all, p0 + sw.units - 1, shares));
-    float* dst = a.out + w * HD + lane * E;
+    float* dst = a.out + (long)w * HD + lane * E;
     float o[E], l = 1.f;
     if (w1 == w2) {
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = dst[e];
     } else {
-        const int at = rho % tile_rows, used = w2 - w1 + 1;
+        const int at = rho & (tile_rows - 1), used = w2 - w1 + 1;
         // the part's first share has it last, the others first
         auto slot = [&](int j) { return (long)(j == 0 ? 2 * w1 + 1 : 2 * (w1 + j)) * tile_rows + at; };
         const float2 none = make_float2(-INFINITY, 0.f);
@@ -1054,7 +1067,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
 #pragma unroll
         for (int off = 16 / E; off > 0; off >>= 1) amax = fmaxf(amax, __shfl_xor(amax, off, 64));
         const float id = amax > 0.f ? 127.f / amax : 0.f;
-        uint8_t* blk = a.outq8 + (w * (HD / 32) + lane * E / 32) * Q8_0_BYTES;
+        uint8_t* blk = a.outq8 + ((long)w * (HD / 32) + lane * E / 32) * Q8_0_BYTES;
 #pragma unroll
         for (int e = 0; e < E; e++) {
             const float r = fminf(fmaxf(rintf(o[e] * id), -128.f), 127.f);
@@ -1174,37 +1187,66 @@ __device__ __forceinline__ ForkSeq fork_seq(const KvForkArgs& a, int i) {
 
 __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
     __shared__ int red[kForkThreads / 64 + 1];
+    __shared__ int src_of[kForkThreads], full_of[kForkThreads];  // of the first outputs
     __shared__ int copies;
-    const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
+    const int t = threadIdx.x;
     int* first = a.scratch;             // n_pages: lowest output that ends in the page
     int* free_list = first + a.n_pages;  // n_pages
     int* copy = free_list + a.n_pages;  // n_out x {source page, destination page, rows}
     if (t == 0) copies = 0;
+    const ForkSeq mine = t < a.n_out ? fork_seq(a, t) : ForkSeq{-1, 0, 0, 0};
+    src_of[t] = mine.src;
+    full_of[t] = mine.full;
+    auto seq_of = [&](int i) { return i == t ? mine : fork_seq(a, i); };
     if (a.refs_out != a.refs)
         for (int p = t; p < a.n_pages; p += kForkThreads) st_dev(a.refs_out + p, a.refs[p]);
     __syncthreads();
-    // what the input rows hold is let go, what the outputs share is taken
-    for (long e = t; e < (long)a.n_in * a.table_ld; e += kForkThreads) {
-        const int p = a.table[e];
-        if (p >= 0 && p < a.n_pages) atomicAdd(a.refs_out + p, -1);
+    // what the input rows hold is let go, what the outputs share is taken; U entries'
+    // loads are in flight together
+    constexpr int U = 4;
+    const long n_old = (long)a.n_in * a.table_ld, n_new = (long)a.n_out * a.table_ld;
+    for (long e0 = t; e0 < n_old; e0 += U * kForkThreads) {
+        int p[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long e = e0 + u * kForkThreads;
+            p[u] = e < n_old ? a.table[e] : -1;
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++)
+            if (p[u] >= 0 && p[u] < a.n_pages) atomicAdd(a.refs_out + p[u], -1);
     }
-    for (int i = wave; i < a.n_out; i += kForkThreads / 64) {
-        const ForkSeq f = fork_seq(a, i);
-        for (int col = lane; col < a.table_ld; col += 64) {
-            int v = -1;
-            if (col < f.full) {
-                const int p = a.table[(long)f.src * a.table_ld + col];
-                if (p >= 0 && p < a.n_pages) {
-                    v = p;
-                    atomicAdd(a.refs_out + p, 1);
-                }
+    for (long e0 = t; e0 < n_new; e0 += U * kForkThreads) {
+        int p[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long e = e0 + u * kForkThreads;
+            p[u] = -1;
+            if (e >= n_new) continue;
+            const int i = (int)div_whole(e, a.table_ld), col = (int)(e - (long)i * a.table_ld);
+            int src, full;
+            if (i < kForkThreads) {
+                src = src_of[i];
+                full = full_of[i];
+            } else {
+                const ForkSeq f = fork_seq(a, i);
+                src = f.src;
+                full = f.full;
             }
-            a.table_out[(long)i * a.table_ld + col] = v;
+            if (col < full) p[u] = a.table[(long)src * a.table_ld + col];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const long e = e0 + u * kForkThreads;
+            if (e >= n_new) continue;
+            const bool page = p[u] >= 0 && p[u] < a.n_pages;
+            if (page) atomicAdd(a.refs_out + p[u], 1);
+            a.table_out[e] = page ? p[u] : -1;
         }
     }
     // pages that an output ends in: the lowest output there may keep it
     for (int i = t; i < a.n_out; i += kForkThreads) {
-        const ForkSeq f = fork_seq(a, i);
+        const ForkSeq f = seq_of(i);
         int p = -1;
         if (f.tail) {
             p = a.table[(long)f.src * a.table_ld + f.full];
@@ -1228,7 +1270,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         const int i = i0 + t;
         int c = 0, keep = 0;
         if (i < a.n_out) {
-            const ForkSeq f = fork_seq(a, i);
+            const ForkSeq f = seq_of(i);
             keep = copy[3 * i + 2];
             if (keep) {
                 const int p = copy[3 * i];
@@ -1247,18 +1289,28 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         want += sum;
     }
     __syncthreads();
+    // the free pages in order, four a thread and round
     int n_free = 0;
-    for (int p0 = 0; p0 < a.n_pages; p0 += kForkThreads) {
-        const int p = p0 + t;
-        const int is = p < a.n_pages && ld_dev(a.refs_out + p) == 0;
-        int sum;
-        const int at = n_free + block_scan(is, red, &sum);
-        if (is && at < want) free_list[at] = p;
+    for (int p0 = 0; p0 < a.n_pages; p0 += 4 * kForkThreads) {
+        const int p = p0 + 4 * t;
+        int is[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) is[u] = p + u < a.n_pages ? ld_dev(a.refs_out + p + u) : 1;
+        int mine_free = 0, sum;
+#pragma unroll
+        for (int u = 0; u < 4; u++) mine_free += is[u] == 0;
+        int at = n_free + block_scan(mine_free, red, &sum);
+#pragma unroll
+        for (int u = 0; u < 4; u++)
+            if (is[u] == 0) {
+                if (at < want) free_list[at] = p + u;
+                at++;
+            }
         n_free += sum;
     }
     __syncthreads();
     for (int i = t; i < a.n_out; i += kForkThreads) {
-        const ForkSeq f = fork_seq(a, i);
+        const ForkSeq f = seq_of(i);
         const int src = copy[3 * i], keep = copy[3 * i + 2];
         int at = copy[3 * i + 1], dst = -1;
         for (int col = f.full + keep; col < f.need; col++, at++) {
@@ -1300,48 +1352,63 @@ __global__ __launch_bounds__(256) void k_kv_copy(uint8_t* k, uint8_t* v, const i
 }
 
 // ---- compaction -----------------------------------------------------------------
-// Workgroup (sequence, layer, K or V): each thread owns 16-byte columns and
-// moves rows in path order.  path[i] >= i and ascending, so no row is written before
-// it was read.
+// Length of a path: it ascends, below 64.  A wave's lanes look at an entry each.
+__device__ __forceinline__ int path_length(const int* way, int most) {
+    const int lane = threadIdx.x & 63;
+    const int v = lane < most ? way[lane] : -1, before = __shfl_up(v, 1, 64);
+    const bool good = lane < most && v < 64 && v > (lane ? before : -1);
+    const uint64_t bad = __ballot(!good);
+    return bad ? __builtin_ctzll(bad) : 64;
+}
+
+// Workgroup (sequence, layer, K or V): each thread owns 16-byte columns and moves rows in
+// path order, eight reads at a time.  path[i] >= i and ascending: a row is written
+// only after every read of it (an earlier write goes to a lower row than every later read).
 __global__ __launch_bounds__(256) void k_kv_compact(uint8_t* k, uint8_t* v, int* len_out,
                                                     const int* table, int table_ld,
                                                     const int* len, const int* path,
                                                     const int* n_path, int max_path, long row_bytes,
-                                                    int n_pages, int page_shift) {
-    const int s = blockIdx.x;
+                                                    int n_pages, int page_shift, int write_len) {
+    constexpr int U = 8;
+    __shared__ int from[64], to[64];
+    const int s = blockIdx.x, t = threadIdx.x;
     const int held = kv_len(len[s], table_ld, page_shift);
     const int* way = path + (long)s * max_path;
-    const int most = min(max(n_path[s], 0), max_path);
-    int n = 0;
-    for (int last = -1; n < most && way[n] > last && way[n] < 64; n++) last = way[n];
+    const int n = path_length(way, min(max(n_path[s], 0), max_path));
+    const int* row = table + (long)s * table_ld;
+    if (t < n) {
+        const int w = way[t];
+        from[t] = (int)kv_row(held + w, row, table_ld, n_pages, page_shift);
+        to[t] = w == t ? -1 : (int)kv_row(held + t, row, table_ld, n_pages, page_shift);
+    }
+    if (write_len && t == 0 && blockIdx.y == 0 && blockIdx.z == 0) len_out[s] = held + n;
+    __syncthreads();
     uint8_t* pool = (blockIdx.z ? v : k) +
                     (((long)blockIdx.y * n_pages) << page_shift) * row_bytes;
-    const int* row = table + (long)s * table_ld;
-    for (long b = threadIdx.x * 16; b < row_bytes; b += 4096) {
-        for (int i = 0; i < n; i++) {
-            if (way[i] == i) continue;
-            const long from = kv_row(held + way[i], row, table_ld, n_pages, page_shift);
-            const long to = kv_row(held + i, row, table_ld, n_pages, page_shift);
-            if (from < 0 || to < 0) continue;
-            *reinterpret_cast<uint4*>(pool + to * row_bytes + b) =
-                *reinterpret_cast<const uint4*>(pool + from * row_bytes + b);
+    for (long b = t * 16; b < row_bytes; b += 4096) {
+        for (int i0 = 0; i0 < n; i0 += U) {
+            uint4 x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (i0 + u < n && from[i0 + u] >= 0 && to[i0 + u] >= 0)
+                    x[u] = *reinterpret_cast<const uint4*>(pool + from[i0 + u] * row_bytes + b);
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (i0 + u < n && from[i0 + u] >= 0 && to[i0 + u] >= 0)
+                    *reinterpret_cast<uint4*>(pool + to[i0 + u] * row_bytes + b) = x[u];
         }
     }
 }
 
-// len_out after the moves (it may be len): in a launch of its own, behind every
-// workgroup that reads len.
+// len_out where it is len (or nothing moves): behind every workgroup that reads len.
 __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int* len,
                                                         const int* path, const int* n_path,
                                                         int n_seq, int max_path, int table_ld,
                                                         int page_shift) {
-    const int s = blockIdx.x * 256 + threadIdx.x;
+    const int s = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (s >= n_seq) return;
-    const int* way = path + (long)s * max_path;
-    const int most = min(max(n_path[s], 0), max_path);
-    int n = 0;
-    for (int last = -1; n < most && way[n] > last && way[n] < 64; n++) last = way[n];
-    len_out[s] = kv_len(len[s], table_ld, page_shift) + n;
+    const int n = path_length(path + (long)s * max_path, min(max(n_path[s], 0), max_path));
+    if ((threadIdx.x & 63) == 0) len_out[s] = kv_len(len[s], table_ld, page_shift) + n;
 }
 
 // Query rows of a KV head that a workgroup takes: the fewest that hold them all, so that
@@ -1357,7 +1424,7 @@ int tile_rows(int rows, int head_dim, int kv_type) {
 
 template <int HD, class T>
 hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), HD,
+    const int tr = tile_rows(a.max_tok * a.group, HD,
                              sizeof(T) == 2 ? AXF_TYPE_F16 : AXF_TYPE_F32);
     if (tr == 16) {
         k_attn_paged_few<HD, T><<<a.shares, 64 * kFewWaves, 0, st>>>(a);
@@ -1400,7 +1467,7 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
-    const int rows = a.max_tok * (a.n_heads / a.n_kv_heads), tr = tile_rows(rows, head_dim, kv_type);
+    const int rows = a.max_tok * a.group, tr = tile_rows(rows, head_dim, kv_type);
     const long seqs = a.n_seq < kPlanSeqs ? a.n_seq : kPlanSeqs;
     const long units = (longest + (tr == 16 ? kFewUnit : kManyUnit) - 1) /
                        (tr == 16 ? kFewUnit : kManyUnit) * seqs * a.n_kv_heads * ((rows + tr - 1) / tr);
@@ -1410,13 +1477,13 @@ void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
 }
 
 size_t attn_paged_scratch(const PagedArgs& a, int kv_type, int head_dim) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim, kv_type);
+    const int tr = tile_rows(a.max_tok * a.group, head_dim, kv_type);
     return (kPlanSeqs + 1) * sizeof(long) + (size_t)2 * a.shares * tr * (head_dim + 2) * 4 + 16;
 }
 
 hipError_t launch_attn_paged(const PagedArgs& a, int kv_type, int head_dim, void* scratch,
                              hipStream_t st) {
-    const int tr = tile_rows(a.max_tok * (a.n_heads / a.n_kv_heads), head_dim, kv_type);
+    const int tr = tile_rows(a.max_tok * a.group, head_dim, kv_type);
     for (int s = 0; s < a.n_seq; s += kPlanSeqs) {
         PagedArgs b = a;
         const long row = (long)s * a.max_tok;
@@ -1469,14 +1536,16 @@ hipError_t launch_kv_compact(const axf_kv_pages& kv, int* len_out, const int* ta
                              int max_path, hipStream_t st) {
     const int shift = __builtin_ctz((unsigned)kv.page_rows);
     const long row_bytes = (long)kv.n_kv_heads * kv.head_dim * (kv.type == AXF_TYPE_F32 ? 4 : 2);
+    // len_out can be written by the workgroups that read len only where they are apart
+    const bool apart = len_out + n_seq <= len || len + n_seq <= len_out;
     if (max_path > 0) {
         k_kv_compact<<<dim3(n_seq, kv.n_layers, 2), 256, 0, st>>>(
             static_cast<uint8_t*>(kv.k), static_cast<uint8_t*>(kv.v), len_out, table, table_ld, len,
-            path, n_path, max_path, row_bytes, kv.n_pages, shift);
+            path, n_path, max_path, row_bytes, kv.n_pages, shift, apart);
         hipError_t e = hipGetLastError();
-        if (e != hipSuccess) return e;
+        if (e != hipSuccess || apart) return e;
     }
-    k_kv_compact_len<<<(n_seq + 255) / 256, 256, 0, st>>>(len_out, len, path, n_path, n_seq, max_path,
+    k_kv_compact_len<<<(n_seq + 3) / 4, 256, 0, st>>>(len_out, len, path, n_path, n_seq, max_path,
                                                       table_ld, shift);
     return hipGetLastError();
 }
