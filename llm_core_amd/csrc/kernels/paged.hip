@@ -72,6 +72,7 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 
 constexpr int kStep = 32;  // keys a step: two 16-key tiles
@@ -214,23 +215,25 @@ __device__ __forceinline__ float rows_sum(float x) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-// q elements d .. d+7 (d % 8 == 0) of a row: bias and RoPE; zero for no row.
-template <int HD>
-__device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, int d, float (&x)[8]) {
-    auto ld8 = [](const float* p, float (&v)[8]) {
-        const f32x4_a4 u = *reinterpret_cast<const f32x4_a4*>(p);
-        const f32x4_a4 w = *reinterpret_cast<const f32x4_a4*>(p + 4);
+__device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
+    const f32x4_a4 u = *reinterpret_cast<const f32x4_a4*>(p);
+    const f32x4_a4 w = *reinterpret_cast<const f32x4_a4*>(p + 4);
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            v[e] = u[e];
-            v[4 + e] = w[e];
-        }
-    };
+    for (int e = 0; e < 4; e++) {
+        v[e] = u[e];
+        v[4 + e] = w[e];
+    }
+}
+
+// q elements d .. d+7 (d % 8 == 0) of a row: bias and RoPE by the tables' row pos.
+template <int HD>
+__device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, int d, long pos,
+                                          float (&x)[8]) {
     const float* qr = a.q + row * a.q_ld + h * HD;
-    ld8(qr + d, x);
+    load8(qr + d, x);
     float b[8];
     if (a.bq) {
-        ld8(a.bq + h * HD + d, b);
+        load8(a.bq + h * HD + d, b);
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] += b[e];
     }
@@ -238,19 +241,22 @@ __device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, i
         constexpr int half = HD / 2;
         const int e2 = d < half ? d + half : d - half, f = d < half ? d : e2;
         float y[8], c[8], s[8];
-        ld8(qr + e2, y);
+        load8(qr + e2, y);
+        load8(a.cos_t + pos * half + f, c);
+        load8(a.sin_t + pos * half + f, s);
         if (a.bq) {
-            ld8(a.bq + h * HD + e2, b);
+            load8(a.bq + h * HD + e2, b);
 #pragma unroll
             for (int e = 0; e < 8; e++) y[e] += b[e];
         }
-        const long p = min(max(a.pos[row], 0), a.n_pos - 1);
-        ld8(a.cos_t + p * half + f, c);
-        ld8(a.sin_t + p * half + f, s);
         const float sign = d < half ? -1.f : 1.f;
 #pragma unroll
         for (int e = 0; e < 8; e++) x[e] = fmaf(x[e], c[e], sign * (y[e] * s[e]));
     }
+}
+// The row's position in the RoPE tables.
+__device__ __forceinline__ long q_pos(const PagedArgs& a, long row) {
+    return a.pos ? min(max(a.pos[row], 0), a.n_pos - 1) : 0;
 }
 
 // How the work is split.  A part is one sequence's, KV head's and row tile's walk over
@@ -283,14 +289,16 @@ __device__ __forceinline__ SeqWork seq_work(const SeqLen& n, int G, int tile_row
     return w;
 }
 
-// cum[s]: units before sequence s (cum[n_seq]: all); the first 256 threads.
+// cum[s]: units before sequence s (cum[n_seq]: all), and its lengths; the first 256
+// threads.
 __device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, int unit, long* cum,
-                                          long* part) {
+                                          long* part, SeqLen* lens) {
     const int t = threadIdx.x, lane = t & 63;
     long w = 0;
     if (t < a.n_seq) {
-        const SeqWork k = seq_work(seq_len(a.len, a.n_tok, a.max_tok, t, a.table_ld, a.page_shift),
-                                   a.group, tile_rows, unit);
+        const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, t, a.table_ld, a.page_shift);
+        lens[t] = n;
+        const SeqWork k = seq_work(n, a.group, tile_rows, unit);
         w = k.units * k.tiles * a.n_kv_heads;
     }
 #pragma unroll
@@ -334,12 +342,15 @@ struct Span {
 };
 
 // The stretch at unit lo of a share that ends at hi; moves lo behind it.
-__device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, int tile_rows, int unit,
-                                          int share, int& s, long& lo, long hi) {
+__device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, const SeqLen* lens,
+                                          int tile_rows, int unit, int share, int& s, long& lo,
+                                          long hi) {
     while (lo >= uniform(cum[s + 1])) s++;
     Span p;
     p.s = s;
-    const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, p.s, a.table_ld, a.page_shift);
+    SeqLen n = lens[s];
+    n.held = __builtin_amdgcn_readfirstlane(n.held);
+    n.tok = __builtin_amdgcn_readfirstlane(n.tok);
     const SeqWork w = seq_work(n, a.group, tile_rows, unit);
     p.held = n.held;
     p.tok = n.tok;
@@ -415,24 +426,18 @@ __device__ __forceinline__ void row_careful(const PagedArgs& a, int s, int i, in
 }
 
 // q's fragments of one 16-row tile: lane's row, elements 32 c + 8 (lane >> 4) .. +7 of
-// each 32-element chunk.  scale: what scores are multiplied by (with F16 pages the
-// row was scaled to the top of fp16's range).
+// each 32-element chunk.  A row past the last takes the first's values (its results go
+// nowhere).  scale: what scores are multiplied by (with F16 pages the row was scaled to
+// the top of fp16's range).
 template <int HD, class T>
-__device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, bool live,
+__device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int rho, long pos,
                                        uint4 (&qf)[HD / 32][Parts<T>::QP], float& scale) {
     constexpr int NC = HD / 32;
-    const int g = (threadIdx.x & 63) >> 4, G = a.group;
-    const int i = rho / G, h = sp.kvh * G + rho % G;
+    const int g = (threadIdx.x & 63) >> 4, i = rho / a.group, h = sp.kvh * a.group + rho - i * a.group;
     float x[NC][8];
 #pragma unroll
-    for (int c = 0; c < NC; c++) {
-        if (live) {
-            q_values8<HD>(a, (long)sp.s * a.max_tok + i, h, 32 * c + 8 * g, x[c]);
-        } else {
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[c][e] = 0.f;
-        }
-    }
+    for (int c = 0; c < NC; c++)
+        q_values8<HD>(a, (long)sp.s * a.max_tok + i, h, 32 * c + 8 * g, pos, x[c]);
     constexpr float kRoot = HD == 64 ? 8.f : HD == 256 ? 16.f : 11.3137084989847603904f;
     scale = kLog2e / kRoot;
     float up = 1.f;
@@ -443,8 +448,8 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int r
 #pragma unroll
             for (int e = 0; e < 8; e++) top = fmaxf(top, fabsf(x[c][e]));
         top = rows_max(top);
-        // 2^(14 - exponent): the largest value between 2^14 and 2^15
-        const int ex = top > 0.f ? min(max(14 - (int)__builtin_amdgcn_frexp_expf(top) + 1, -100), 100) : 0;
+        // 2^(15 - exponent): the largest value between 2^14 and 2^15
+        const int ex = top > 0.f ? min(max(15 - (int)__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
         up = __builtin_ldexpf(1.f, ex);
         scale = __builtin_ldexpf(scale, -ex);
     }
@@ -521,9 +526,10 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     __shared__ float os[kFewWaves][16][HD + 4];
     __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
     __shared__ long cum[kPlanSeqs + 1], scan[4];
+    __shared__ SeqLen lens[kPlanSeqs];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int n = lane & 15, g = lane >> 4, G = a.group;
-    make_plan(a, 16, kFewUnit, cum, scan);
+    make_plan(a, 16, kFewUnit, cum, scan, lens);
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s <= a.n_seq; s += 256) a.plan[s] = cum[s];
     const long all = uniform(cum[a.n_seq]);
@@ -534,7 +540,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
     while (lo < hi) {
-    const Span sp = next_span(a, cum, 16, kFewUnit, share, seq, lo, hi);
+    const Span sp = next_span(a, cum, lens, 16, kFewUnit, share, seq, lo, hi);
     const int kvh = sp.kvh, tile = sp.tile, rows = sp.rows;
     const int rho = tile * 16 + n;
     const bool live = rho < rows;
@@ -579,8 +585,12 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     };
     const int first = sp.j0 + wave * kStep, hop = kFewWaves * kStep;
     int r[2], rn[2], pg[2];
+    const int rq = live ? rho : 0, iq = rq / G;
+    const long rowq = (long)sp.s * a.max_tok + iq;
+    pages_of(min(first, sp.j1 - 1), pg);
+    const long pos = q_pos(a, rowq);
+    const uint64_t mask = seen_mask(a, rowq, iq);
     if (first < sp.j1) {
-        pages_of(first, pg);
         rows_of(first, pg, r);
         load_k(r);
         load_v(r);
@@ -588,8 +598,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
     }
     uint4 qf[NC][QP];
     float scale;
-    load_q<HD, T>(a, sp, rho, live, qf, scale);
-    const uint64_t mask = live ? seen_mask(a, (long)sp.s * a.max_tok + rho / G, rho / G) : 0;
+    load_q<HD, T>(a, sp, rq, pos, qf, scale);
     f32x4 o[ND];
 #pragma unroll
     for (int d = 0; d < ND; d++) o[d] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -611,9 +620,9 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
                 else
                     Parts<T>::split_kv(kr[t][c2], kf[t]);
             }
-            const uint4* const q[1] = {qf[c2]};
+            const uint4* const qc[1] = {qf[c2]};
             f32x4* const to[2][1] = {{st[0]}, {st[1]}};
-            Parts<T>::template scores<2, 1>(kf, q, to);
+            Parts<T>::template scores<2, 1>(kf, qc, to);
         }
         // no row behind a key: only bad tables have such keys before j1
         const bool hole = __any(r[0] < 0 || r[1] < 0);
@@ -741,9 +750,10 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     __shared__ uint64_t masks[TR];
     __shared__ uint32_t holes[NB];  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
     __shared__ long cum[kPlanSeqs + 1], scan[4];
+    __shared__ SeqLen lens[kPlanSeqs];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, g = lane >> 4, G = a.group;
-    make_plan(a, TR, kManyUnit, cum, scan);
+    make_plan(a, TR, kManyUnit, cum, scan, lens);
     if (blockIdx.x == 0)
         for (int s = t; s <= a.n_seq; s += 64 * NW) a.plan[s] = cum[s];
     const long all = uniform(cum[a.n_seq]);
@@ -754,7 +764,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
     while (lo < hi) {
-    const Span sp = next_span(a, cum, TR, kManyUnit, share, seq, lo, hi);
+    const Span sp = next_span(a, cum, lens, TR, kManyUnit, share, seq, lo, hi);
     const int kvh = sp.kvh, rows = sp.rows, row0 = sp.tile * TR;
     const long ld = (long)a.n_kv_heads * HD;
 
@@ -860,7 +870,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     for (int w = 0; w < MW; w++) {
         const int rho = row0 + (wave + NW * w) * 16 + n;
         act[w] = row0 + (wave + NW * w) * 16 < rows;
-        load_q<HD, T>(a, sp, rho, rho < rows, qf[w], scale[w]);
+        const int rq = rho < rows ? rho : 0;
+        load_q<HD, T>(a, sp, rq, q_pos(a, (long)sp.s * a.max_tok + rq / G), qf[w], scale[w]);
         m[w] = -INFINITY;
         l[w] = 0.f;
 #pragma unroll
@@ -1085,52 +1096,57 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
     constexpr int PER = HD / 8;  // threads a head
     const int per_row = a.n_kv_heads * PER;
     const long t = (long)blockIdx.x * 256 + threadIdx.x;
-    const long row = t / per_row;
+    const long row = div_whole(t, per_row);
     if (row >= (long)a.n_seq * a.max_tok) return;
-    const int s = (int)(row / a.max_tok), i = (int)(row % a.max_tok);
+    const int s = (int)((uint32_t)row / (uint32_t)a.max_tok), i = (int)row - s * a.max_tok;
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
     if (i >= n.tok) return;
-    const long r = kv_row(n.held + i, a.table + (long)s * a.table_ld, a.table_ld, a.n_pages,
-                          a.page_shift);
-    if (r < 0) return;
-    const int u = (int)(t % per_row), h = u / PER, d = (u % PER) * 4;
+    const int u = (int)(t - row * per_row), h = u / PER, d = (u % PER) * 4;
     const int at = h * HD + d;
+    // every load before the first use of one
+    const int page = kv_page(n.held + i, a.table + (long)s * a.table_ld, a.table_ld, a.page_shift);
+    const long p = a.pos ? min(max(a.pos[row], 0), a.n_pos - 1) : 0;
+    auto ld4 = [](const float* q) { return *reinterpret_cast<const f32x4_a4*>(q); };
+    f32x4_a4 x = ld4(a.xk + row * a.k_ld + at), y = ld4(a.xk + row * a.k_ld + at + HD / 2);
+    f32x4_a4 z = ld4(a.xv + row * a.v_ld + at), w = ld4(a.xv + row * a.v_ld + at + HD / 2);
+    if (a.bk) {
+        x += ld4(a.bk + at);
+        y += ld4(a.bk + at + HD / 2);
+    }
+    if (a.bv) {
+        z += ld4(a.bv + at);
+        w += ld4(a.bv + at + HD / 2);
+    }
+    if (a.pos) {
+        const f32x4_a4 c = ld4(a.cos_t + p * (HD / 2) + d), sn = ld4(a.sin_t + p * (HD / 2) + d);
+        const f32x4_a4 x0 = x;
+        x = x0 * c - y * sn;
+        y = y * c + x0 * sn;
+    }
+    const long r = kv_row_of(n.held + i, page, a.table_ld, a.n_pages, a.page_shift);
+    if (r < 0) return;
     T* k = static_cast<T*>(a.k) + r * a.n_kv_heads * HD + at;
     T* v = static_cast<T*>(a.v) + r * a.n_kv_heads * HD + at;
-    const float* xk = a.xk + row * a.k_ld + at;
-    const float* xv = a.xv + row * a.v_ld + at;
-    const long p = a.pos ? min(max(a.pos[row], 0), a.n_pos - 1) : 0;
+    auto st4 = [](T* q, const f32x4_a4& f) {  // F16 pages: to nearest, ties to even
+        T o[4];
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        float x = xk[e], y = xk[e + HD / 2], z = xv[e], w = xv[e + HD / 2];
-        if (a.bk) {
-            x += a.bk[at + e];
-            y += a.bk[at + e + HD / 2];
-        }
-        if (a.bv) {
-            z += a.bv[at + e];
-            w += a.bv[at + e + HD / 2];
-        }
-        if (a.pos) {
-            const float c = a.cos_t[p * (HD / 2) + d + e], sn = a.sin_t[p * (HD / 2) + d + e];
-            const float x0 = x;
-            x = x0 * c - y * sn;
-            y = y * c + x0 * sn;
-        }
-        // F16 pages: to nearest, ties to even
-        k[e] = (T)x;
-        k[e + HD / 2] = (T)y;
-        v[e] = (T)z;
-        v[e + HD / 2] = (T)w;
-    }
+        for (int e = 0; e < 4; e++) o[e] = (T)f[e];
+        __builtin_memcpy(__builtin_assume_aligned(q, 4 * sizeof(T)), o, sizeof(o));
+    };
+    st4(k, x);
+    st4(k + HD / 2, y);
+    st4(v, z);
+    st4(v + HD / 2, w);
 }
 
 // ---- fork --------------------------------------------------------------------
 // The tables are small (some ten thousand entries), so one workgroup walks them with
-// barriers between its steps and no other launch: reference counts as device-scope
-// atomics (whole numbers, so their order does not matter), everything else by
-// index order.
+// barriers between its steps and no other launch.  Reference counts are atomics (whole
+// numbers, so their order does not matter), in LDS up to kForkLdsPages pages: one CU's
+// scattered atomics to L2 go one a cycle or less, 128 sequences of 49 pages took 19 us
+// with them.  Everything else goes by index order.
 constexpr int kForkThreads = 1024;
+constexpr int kForkLdsPages = 32768;  // 128 KiB
 
 __device__ __forceinline__ int ld_dev(const int* p) {
     return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
@@ -1185,7 +1201,9 @@ __device__ __forceinline__ ForkSeq fork_seq(const KvForkArgs& a, int i) {
     return f;
 }
 
+template <bool kLds>
 __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
+    extern __shared__ int lds_refs[];
     __shared__ int red[kForkThreads / 64 + 1];
     __shared__ int src_of[kForkThreads], full_of[kForkThreads];  // of the first outputs
     __shared__ int copies;
@@ -1198,8 +1216,13 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
     src_of[t] = mine.src;
     full_of[t] = mine.full;
     auto seq_of = [&](int i) { return i == t ? mine : fork_seq(a, i); };
-    if (a.refs_out != a.refs)
+    auto add_ref = [&](int p, int v) { atomicAdd(kLds ? lds_refs + p : a.refs_out + p, v); };
+    auto ref_of = [&](int p) { return kLds ? lds_refs[p] : ld_dev(a.refs_out + p); };
+    if (kLds) {
+        for (int p = t; p < a.n_pages; p += kForkThreads) lds_refs[p] = a.refs[p];
+    } else if (a.refs_out != a.refs) {
         for (int p = t; p < a.n_pages; p += kForkThreads) st_dev(a.refs_out + p, a.refs[p]);
+    }
     __syncthreads();
     // what the input rows hold is let go, what the outputs share is taken; U entries'
     // loads are in flight together
@@ -1214,7 +1237,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         }
 #pragma unroll
         for (int u = 0; u < U; u++)
-            if (p[u] >= 0 && p[u] < a.n_pages) atomicAdd(a.refs_out + p[u], -1);
+            if (p[u] >= 0 && p[u] < a.n_pages) add_ref(p[u], -1);
     }
     for (long e0 = t; e0 < n_new; e0 += U * kForkThreads) {
         int p[U];
@@ -1240,7 +1263,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
             const long e = e0 + u * kForkThreads;
             if (e >= n_new) continue;
             const bool page = p[u] >= 0 && p[u] < a.n_pages;
-            if (page) atomicAdd(a.refs_out + p[u], 1);
+            if (page) add_ref(p[u], 1);
             a.table_out[e] = page ? p[u] : -1;
         }
     }
@@ -1261,7 +1284,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
     __syncthreads();
     for (int i = t; i < a.n_out; i += kForkThreads) {
         const int p = copy[3 * i];
-        copy[3 * i + 2] = p >= 0 && ld_dev(first + p) == i && ld_dev(a.refs_out + p) == 0;
+        copy[3 * i + 2] = p >= 0 && ld_dev(first + p) == i && ref_of(p) == 0;
     }
     __syncthreads();
     // the kept ones counted; each output's place among the pages to take
@@ -1274,7 +1297,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
             keep = copy[3 * i + 2];
             if (keep) {
                 const int p = copy[3 * i];
-                atomicAdd(a.refs_out + p, 1);
+                add_ref(p, 1);
                 a.table_out[(long)i * a.table_ld + f.full] = p;
             }
             c = max(0, f.need - f.full - keep);
@@ -1295,7 +1318,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         const int p = p0 + 4 * t;
         int is[4];
 #pragma unroll
-        for (int u = 0; u < 4; u++) is[u] = p + u < a.n_pages ? ld_dev(a.refs_out + p + u) : 1;
+        for (int u = 0; u < 4; u++) is[u] = p + u < a.n_pages ? ref_of(p + u) : 1;
         int mine_free = 0, sum;
 #pragma unroll
         for (int u = 0; u < 4; u++) mine_free += is[u] == 0;
@@ -1316,7 +1339,7 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         for (int col = f.full + keep; col < f.need; col++, at++) {
             const int p = at < n_free ? free_list[at] : -1;
             a.table_out[(long)i * a.table_ld + col] = p;
-            if (p >= 0) st_dev(a.refs_out + p, 1);
+            if (p >= 0) add_ref(p, 1);  // nothing held it
             if (col == f.full) dst = p;
         }
         const bool copied = src >= 0 && dst >= 0;
@@ -1326,6 +1349,8 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
         if (copied) atomicAdd(&copies, 1);
     }
     __syncthreads();
+    if (kLds)
+        for (int p = t; p < a.n_pages; p += kForkThreads) a.refs_out[p] = lds_refs[p];
     if (t == 0) {
         a.info[0] = copies;
         a.info[1] = max(0, want - n_free);
@@ -1387,15 +1412,17 @@ __global__ __launch_bounds__(256) void k_kv_compact(uint8_t* k, uint8_t* v, int*
                     (((long)blockIdx.y * n_pages) << page_shift) * row_bytes;
     for (long b = t * 16; b < row_bytes; b += 4096) {
         for (int i0 = 0; i0 < n; i0 += U) {
-            uint4 x[U];
+            u32x4 x[U];  // read also where nothing moves: no branch between the reads
 #pragma unroll
             for (int u = 0; u < U; u++)
-                if (i0 + u < n && from[i0 + u] >= 0 && to[i0 + u] >= 0)
-                    x[u] = *reinterpret_cast<const uint4*>(pool + from[i0 + u] * row_bytes + b);
+                x[u] = *reinterpret_cast<const u32x4*>(
+                    pool + (long)max(from[min(i0 + u, n - 1)], 0) * row_bytes + b);
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (i0 + u < n && from[i0 + u] >= 0 && to[i0 + u] >= 0)
-                    *reinterpret_cast<uint4*>(pool + to[i0 + u] * row_bytes + b) = x[u];
+            for (int u = 0; u < U; u++) {
+                const int i = min(i0 + u, n - 1);
+                if (i0 + u < n && from[i] >= 0 && to[i] >= 0)
+                    *reinterpret_cast<u32x4*>(pool + (long)to[i] * row_bytes + b) = x[u];
+            }
         }
     }
 }
@@ -1520,7 +1547,10 @@ size_t kv_fork_scratch(int n_pages, int n_out) {
 }
 
 hipError_t launch_kv_fork(const KvForkArgs& a, const axf_kv_pages& kv, hipStream_t st) {
-    k_kv_fork<<<1, kForkThreads, 0, st>>>(a);
+    if (a.n_pages <= kForkLdsPages)
+        k_kv_fork<true><<<1, kForkThreads, a.n_pages * sizeof(int), st>>>(a);
+    else
+        k_kv_fork<false><<<1, kForkThreads, 0, st>>>(a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.extra == 0 || a.n_out == 0) return e;
     const long row_bytes = (long)kv.n_kv_heads * kv.head_dim * (kv.type == AXF_TYPE_F32 ? 4 : 2);
