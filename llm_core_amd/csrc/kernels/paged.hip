@@ -1489,8 +1489,12 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 
 }  // namespace
 
-// Workgroups of the launch: as many as run at once (two of 4 waves a CU, one of 8), or as
-// few as have a unit each by the caller's estimate of the lengths.
+// Workgroups of the launch: as many as run at once, or as few as have a unit each by the
+// caller's estimate of the lengths.  A CU holds two workgroups of 64-row tiles, or of few
+// rows at 64 elements a head (fewer than 256 registers); one of few rows at 128 and 256
+// elements, or of 8 waves.  More than run at once leave the last ones a CU to
+// themselves: 16 sequences of 32/8 heads @4000 with 256, 512, 1024 workgroups: 73, 83,
+// 98 us.
 void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
@@ -1498,7 +1502,7 @@ void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long seqs = a.n_seq < kPlanSeqs ? a.n_seq : kPlanSeqs;
     const long units = (longest + (tr == 16 ? kFewUnit : kManyUnit) - 1) /
                        (tr == 16 ? kFewUnit : kManyUnit) * seqs * a.n_kv_heads * ((rows + tr - 1) / tr);
-    const long most = tr > 64 ? 256 : 512;
+    const long most = tr == 64 || (tr == 16 && head_dim == 64) ? 512 : 256;
     const long shares = units < most ? units : most;
     a.shares = (int)((shares + 7) & ~7L);
 }
