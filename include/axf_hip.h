@@ -292,7 +292,7 @@ int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n)
  *   - parent[i] outside 0..n_in-1 or len[i] < 0: sequence i holds nothing.
  * A text starts as an input row of -1 with len 0.  table_out: n_out rows of
  * table_ld entries, entries past the room -1, not the array `table`.  refs_out
- * (n_pages) may be refs.  info (3 int32): copied pages, entries left without a
+ * (n_pages) may be refs; refs has to count what the tables hold.  info (3 int32): copied pages, entries left without a
  * page, pages free afterwards.  Room past table_ld pages is cut off there. */
 int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, int32_t* refs_out,
                     int32_t* info, const int32_t* table, const int32_t* refs, int n_in,
@@ -320,8 +320,10 @@ int axf_hip_kv_store(axf_ctx* ctx, const axf_kv_pages* kv, int layer, const int3
  * axf_hip_kv_store (pos NULL: already turned).  out row (s, i) of n_heads *
  * head_dim floats, outq8 (may be NULL) its Q8_0 blocks; a row that sees nothing
  * is zero, rows i >= n_tok[s] are left as they were.  What a masked place holds
- * (NaN and infinities too) changes nothing.  max_len: about the longest len[s],
- * for the split of the work; any value gives the same sums up to their order. */
+ * (NaN and infinities too) changes nothing; a score of -inf has no weight, one of
+ * +inf or NaN makes its row NaN.  out is apart from q.  max_len: about the longest
+ * len[s], for the split of the work; any value gives the same sums up to their
+ * order.  Held in fp32 throughout. */
 int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, int q_ld,
                        const float* bq, const axf_kv_pages* kv, int layer, const int32_t* table,
                        int table_ld, const int32_t* len, const int32_t* n_tok,
@@ -332,7 +334,8 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
 /* After a drafted tree was verified: rows len[s] + path[s * max_path + i] move to
  * len[s] + i for i < n_path[s], in all layers, and len_out[s] = len[s] + n_path[s]
  * (len_out may be len).  A path ascends (0 <= path[0] < path[1] < ...), as a
- * tree's ways down do; it ends before an entry that does not.  max_path <= 64. */
+ * tree's ways down do; it ends before an entry that does not.  max_path <= 64.
+ * Moved rows lie in pages of their sequence alone (axf_hip_kv_fork with extra). */
 int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
                        const int32_t* table, int table_ld, const int32_t* len,
                        const int32_t* path, const int32_t* n_path, int n_seq, int max_path);
@@ -345,8 +348,8 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
  * one continuation, eos_id, that keeps its score.  A score of -inf or NaN (a
  * masked token, an unused beam with cum -inf; a row with a NaN or +inf logit) is
  * no continuation.  token, parent (the beam, 0..n_beams-1) and score: n_out a
- * sequence, best first; -1, -1 and -inf where there are no more.  n_beams and
- * n_out up to 64, n_vocab up to 2^26. */
+ * sequence, best first; -1, -1 and -inf where there are no more; with n_out =
+ * n_beams score may be cum.  n_beams and n_out up to 64, n_vocab up to 2^26. */
 int axf_hip_beam_select(axf_ctx* ctx, int32_t* token, int32_t* parent, float* score,
                         const float* logits, int ld, const float* cum, const int32_t* done,
                         int eos_id, int n_seq, int n_beams, int n_vocab, int n_out);

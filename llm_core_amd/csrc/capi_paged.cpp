@@ -31,6 +31,12 @@ size_t layer_bytes(const axf_kv_pages* kv) {
            (kv->type == AXF_TYPE_F32 ? 4 : 2);
 }
 
+// Whether two arrays have memory in common.
+bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
 // Positions are 32-bit.
 bool table_ok(const axf_kv_pages* kv, int table_ld) {
     return table_ld > 0 && ((long)table_ld << page_shift(kv)) <= (1L << 30);
@@ -67,9 +73,11 @@ int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, in
     AXF_REQUIRE(refs && refs_out && info && (n_in == 0 || table) &&
                     (n_out == 0 || (table_out && parent && len)),
                 "null pointer");
-    AXF_REQUIRE(n_in == 0 || n_out == 0 || table_out + (size_t)n_out * table_ld <= table ||
-                    table + (size_t)n_in * table_ld <= table_out,
+    AXF_REQUIRE(!overlap(table_out, (size_t)n_out * table_ld * 4, table, (size_t)n_in * table_ld * 4),
                 "table_out must not overlap table");
+    AXF_REQUIRE(refs_out == refs ||
+                    !overlap(refs_out, (size_t)kv->n_pages * 4, refs, (size_t)kv->n_pages * 4),
+                "refs_out must be refs or apart from it");
     AXF_REQUIRE(aligned(table, 4) && aligned(table_out, 4) && aligned(refs, 4) &&
                     aligned(refs_out, 4) && aligned(info, 4) && aligned(parent, 4) &&
                     aligned(len, 4),
@@ -163,6 +171,10 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
     AXF_REQUIRE(out && q && table && len, "null pointer");
     AXF_REQUIRE(!pos || (cos_t && sin_t && n_pos > 0), "pos needs the RoPE tables");
     AXF_REQUIRE(q_ld >= n_heads * kv->head_dim, "q_ld below one row");
+    const size_t rows = (size_t)n_seq * max_tok;
+    AXF_REQUIRE(!overlap(out, rows * n_heads * kv->head_dim * 4, q,
+                         ((rows - 1) * q_ld + (size_t)n_heads * kv->head_dim) * 4),
+                "out must not overlap q");
     AXF_REQUIRE(aligned(out, 4) && aligned(outq8, 4) && aligned(q, 4) && aligned(bq, 4) &&
                     aligned(table, 4) && aligned(len, 4) && aligned(n_tok, 4) &&
                     aligned(mask, 8) && aligned(pos, 4) && aligned(cos_t, 4) && aligned(sin_t, 4),
@@ -210,6 +222,8 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
     AXF_REQUIRE(n_seq >= 0 && n_seq <= 65535, "bad n_seq");
     if (n_seq == 0) return AXF_OK;
     AXF_REQUIRE(len_out && table && len && n_path && (path || max_path == 0), "null pointer");
+    AXF_REQUIRE(len_out == len || !overlap(len_out, (size_t)n_seq * 4, len, (size_t)n_seq * 4),
+                "len_out must be len or apart from it");
     AXF_REQUIRE(aligned(len_out, 4) && aligned(table, 4) && aligned(len, 4) && aligned(path, 4) &&
                     aligned(n_path, 4),
                 "misaligned pointer");
@@ -230,6 +244,9 @@ int axf_hip_beam_select(axf_ctx* ctx, int32_t* token, int32_t* parent, float* sc
     AXF_REQUIRE(ld >= n_vocab, "ld below one row");
     if (n_seq == 0) return AXF_OK;
     AXF_REQUIRE(token && parent && score && logits && cum, "null pointer");
+    AXF_REQUIRE((score == cum && n_out == n_beams) ||
+                    !overlap(score, (size_t)n_seq * n_out * 4, cum, (size_t)n_seq * n_beams * 4),
+                "score must be cum (with n_out = n_beams) or apart from it");
     AXF_REQUIRE(!done || (eos_id >= 0 && eos_id < n_vocab), "eos_id out of range");
     AXF_REQUIRE(aligned(token, 4) && aligned(parent, 4) && aligned(score, 4) &&
                     aligned(logits, 4) && aligned(cum, 4) && aligned(done, 4),

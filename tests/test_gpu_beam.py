@@ -143,6 +143,27 @@ def test_all_done(ctx):
     assert got[2].tolist() == [[-1.0, -1.0, -3.0, -np.inf, -np.inf]]
 
 
+def test_scores_over_the_beams_own(ctx):
+    """score is cum: a search's running scores in one array."""
+    rng = np.random.default_rng(7)
+    n, B, V = 9, 5, 4099
+    x = rng.standard_normal((n, B, V)).astype(np.float32)
+    cum = -rng.random((n, B)).astype(np.float32)
+    i0 = np.zeros((n, B), np.int32)
+    with R.Device(ctx) as d:
+        t, p, s = d.up(i0), d.up(i0), d.up(cum)
+        ctx.beam_select(t, p, s, d.up(x), V, s, n, B, V, B)
+        check((d.get(t, i0), d.get(p, i0), d.get(s, cum)), x, cum, None, -1, B)
+
+
+def test_many_rows(ctx):
+    """More rows than a grid's second dimension holds."""
+    rng = np.random.default_rng(8)
+    x = rng.standard_normal((1100, 60, 40)).astype(np.float32)
+    cum = -rng.random((1100, 60)).astype(np.float32)
+    check(run(ctx, x, cum, None, -1, 3), x, cum, None, -1, 3)
+
+
 def test_same_bits_each_time(ctx):
     rng = np.random.default_rng(6)
     x = (rng.standard_normal((4, 8, 32000)) * 2).astype(np.float32)

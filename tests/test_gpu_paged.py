@@ -248,6 +248,25 @@ def test_attn_shared_pages(ctx):
     c.check(c.run(ctx), *c.want())
 
 
+@pytest.mark.parametrize("tok", [1, 3])
+def test_attn_many_sequences(ctx, tok):
+    """More sequences than one launch deals out, some of them empty."""
+    rng = np.random.default_rng(47)
+    n = 700
+    lens = np.where(rng.random(n) < 0.2, 0, rng.integers(0, 60, n))
+    lens[[0, 255, 256, 511, 699]] = [200, 33, 150, 0, 90]
+    n_tok = np.where(rng.random(n) < 0.1, 0, rng.integers(1, tok + 1, n))
+    c = Case(48, 4, 2, 64, "f16", 8, lens.tolist(), n_tok.tolist(), tok, mask=None)
+    c.check(c.run(ctx), *c.want())
+
+
+@pytest.mark.parametrize("heads,tok", [(64, 1), (64, 5), (40, 13)])
+def test_attn_one_kv_head(ctx, heads, tok):
+    """Every query head on one KV head: row tiles of several kinds, partly filled."""
+    c = Case(heads, heads, 1, 64, "f32", 1024, [1500, 20], [tok, max(1, tok - 1)], tok)
+    c.check(c.run(ctx), *c.want())
+
+
 def test_attn_same_bits_each_time(ctx):
     c = Case(29, 32, 8, 128, "f32", 16, [2500, 40], [24, 24], 24)
     a = c.run(ctx)
@@ -422,6 +441,22 @@ def test_fork_tables_of_several_hundred(ctx):
     parent = np.minimum(rng.integers(0, n, n), rng.integers(0, n, n)).astype(np.int32)
     got = run_fork(ctx, 0, np.float32, k, k, table, refs, parent, lens[parent], page, 3)
     assert len(check_fork(got, k, k, table, refs, parent, lens[parent], page, 3)) > 200
+
+
+@pytest.mark.parametrize("n_pages", [32768, 32769])
+def test_fork_large_pools(ctx, n_pages):
+    """Reference counts in LDS and past what LDS holds."""
+    rng = np.random.default_rng(n_pages)
+    n, page, ld = 40, 2, 500
+    lens = rng.integers(0, 900, n).astype(np.int32)
+    table = R.tables(lens, page, ld, n_pages, rng)
+    refs = np.zeros(n_pages, np.int32)
+    np.add.at(refs, table[table >= 0], 1)
+    k = rng.standard_normal((1, n_pages, page, 1, 64)).astype(np.float16)
+    parent = rng.integers(0, n, 60).astype(np.int32)
+    for in_place in (False, True):
+        got = run_fork(ctx, 1, np.float16, k, k, table, refs, parent, lens[parent], page, 5, in_place)
+        check_fork(got, k, k, table, refs, parent, lens[parent], page, 5)
 
 
 def test_fork_partial_page_held_in_full_by_a_sibling(ctx):

@@ -35,12 +35,12 @@ FORK = dict(kv=None, table_out=D, refs_out=D, info=D, table=2 * D, refs=D, n_in=
             n_out=2, table_ld=4, extra=1)
 STORE = dict(kv=None, layer=0, table=D, table_ld=4, len=D, n_tok=D, n_seq=2, max_tok=3, k=D,
              k_ld=256, bk=D, v=D, v_ld=256, bv=D, pos=D, cos=D, sin=D, n_pos=9)
-ATTN = dict(out=D, outq8=D, q=D, q_ld=512, bq=D, kv=None, layer=0, table=D, table_ld=4, len=D,
+ATTN = dict(out=D, outq8=D, q=3 * D, q_ld=512, bq=D, kv=None, layer=0, table=D, table_ld=4, len=D,
             n_tok=D, mask=D, pos=D, cos=D, sin=D, n_pos=9, n_seq=2, max_tok=3, max_len=40,
             n_heads=4)
 COMPACT = dict(kv=None, len_out=D, table=D, table_ld=4, len=D, path=D, n_path=D, n_seq=2,
                max_path=3)
-SELECT = dict(token=D, parent=D, score=D, logits=D, ld=100, cum=D, done=D, eos=2, n_seq=2,
+SELECT = dict(token=D, parent=D, score=D, logits=D, ld=100, cum=2 * D, done=D, eos=2, n_seq=2,
               n_beams=4, n_vocab=100, n_out=8)
 CALLS = {"axf_hip_kv_fork": FORK, "axf_hip_kv_store": STORE, "axf_hip_attn_paged": ATTN,
          "axf_hip_kv_compact": COMPACT, "axf_hip_beam_select": SELECT}
@@ -71,7 +71,8 @@ def test_bad_pools_are_refused(name, bad):
                             dict(table=None), dict(refs=None), dict(n_in=-1), dict(parent=None),
                             dict(len=None), dict(n_out=-1), dict(n_out=70000), dict(table_ld=0),
                             dict(table_ld=1 << 27), dict(extra=-1), dict(table_out=2 * D),
-                            dict(table_out=2 * D + 16), dict(table=2 * D + 2), dict(info=D + 1)],
+                            dict(table_out=2 * D + 16), dict(table_out=2 * D - 16),
+                            dict(refs_out=D + 16), dict(table=2 * D + 2), dict(info=D + 1)],
         "axf_hip_kv_store": [dict(layer=-1), dict(layer=2), dict(table=None), dict(table_ld=0),
                              dict(len=None), dict(n_seq=-1), dict(max_tok=-1),
                              dict(n_seq=1 << 20, max_tok=64), dict(k=None), dict(v=None),
@@ -83,16 +84,18 @@ def test_bad_pools_are_refused(name, bad):
                                dict(max_len=-1), dict(n_seq=65536, max_tok=64, n_heads=32, q_ld=1 << 14),
                                dict(n_heads=0), dict(n_heads=3),
                                dict(n_heads=2048), dict(mask=D + 4), dict(out=D + 2),
-                               dict(outq8=D + 2), dict(q=D + 1)],
+                               dict(outq8=D + 2), dict(q=D + 1), dict(q=D),
+                               dict(q=D + 6 * 2048 - 4), dict(q=D - 4)],
         "axf_hip_kv_compact": [dict(len_out=None), dict(table=None), dict(len=None),
                                dict(path=None), dict(n_path=None), dict(n_seq=-1),
                                dict(n_seq=70000), dict(max_path=65), dict(max_path=-1),
-                               dict(table_ld=-1), dict(path=D + 2)],
+                               dict(table_ld=-1), dict(path=D + 2), dict(len_out=D + 4)],
         "axf_hip_beam_select": [dict(token=None), dict(parent=None), dict(score=None),
                                 dict(logits=None), dict(cum=None), dict(ld=99), dict(n_beams=0),
                                 dict(n_beams=65), dict(n_out=0), dict(n_out=65), dict(n_vocab=0),
                                 dict(n_vocab=(1 << 26) + 1, ld=1 << 27), dict(n_seq=-1),
-                                dict(eos=-1), dict(eos=100), dict(logits=D + 2), dict(done=D + 2)],
+                                dict(eos=-1), dict(eos=100), dict(logits=D + 2), dict(done=D + 2),
+                                dict(score=2 * D), dict(score=2 * D + 4), dict(cum=D)],
     }.items() for b in bads])
 def test_bad_arguments_are_refused(name, bad):
     refused(name, call_args(CALLS[name], **bad))
