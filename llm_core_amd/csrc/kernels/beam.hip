@@ -18,7 +18,7 @@ namespace axf {
 
 namespace {
 
-constexpr int kMergeThreads = 1024;
+constexpr int kMergeThreads = 512;
 
 __device__ __forceinline__ uint32_t ordered32(float v) {
     const uint32_t u = __float_as_uint(v + 0.f);  // -0 and +0 are one logit

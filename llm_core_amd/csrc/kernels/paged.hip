@@ -1026,26 +1026,31 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
         const int at = rho & (tile_rows - 1), used = w2 - w1 + 1;
         // the part's first share has it last, the others first
         auto slot = [&](int j) { return (long)(j == 0 ? 2 * w1 + 1 : 2 * (w1 + j)) * tile_rows + at; };
-        const float2 none = make_float2(-INFINITY, 0.f);
-        float top = -INFINITY;
-        for (int j = lane; j < used; j += 64) top = fmaxf(top, a.part_ml[slot(j)].x);
+        // the sums of shares j0 .. j0 + U - 1, on their way while the weights are found
+        auto sums = [&](int j0, float (&v)[U][E]) {
+#pragma unroll
+            for (int j = 0; j < U; j++)
+#pragma unroll
+                for (int e = 0; e < E; e++)
+                    v[j][e] = a.part[slot(min(j0 + j, used - 1)) * HD + lane * E + e];
+        };
+        float v[U][E];
+        float2 ml = lane < used ? a.part_ml[slot(lane)] : make_float2(-INFINITY, 0.f);
+        sums(0, v);
+        float top = ml.x;
+        for (int j = lane + 64; j < used; j += 64) top = fmaxf(top, a.part_ml[slot(j)].x);
         top = wave_max(top);
         const float base = top == -INFINITY ? 0.f : top;
         l = 0.f;
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] = 0.f;
         for (int b = 0; b < used; b += 64) {
-            const float2 ml = b + lane < used ? a.part_ml[slot(b + lane)] : none;
+            if (b) ml = b + lane < used ? a.part_ml[slot(b + lane)] : make_float2(-INFINITY, 0.f);
             const float f = ml.y == 0.f ? 0.f : __builtin_amdgcn_exp2f(ml.x - base);
             l += wave_sum(ml.y * f);
             const int here = min(64, used - b);
             for (int j0 = 0; j0 < here; j0 += U) {
-                float v[U][E];
-#pragma unroll
-                for (int j = 0; j < U; j++)
-#pragma unroll
-                    for (int e = 0; e < E; e++)
-                        v[j][e] = a.part[slot(b + min(j0 + j, here - 1)) * HD + lane * E + e];
+                if (b + j0) sums(b + j0, v);
 #pragma unroll
                 for (int j = 0; j < U; j++) {
                     const float fj = j0 + j < here ? __uint_as_float(__builtin_amdgcn_readlane(
