@@ -13,11 +13,6 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-template <class T>
-__device__ __forceinline__ float kv_value(T v) {
-    return (float)v;
-}
-
 // The token counts of sequence s, cut to what the call and the table can hold.
 struct SeqLen {
     int held, tok;
@@ -500,12 +495,6 @@ __device__ __forceinline__ void weights(const f32x4 (&st)[2][Parts<T>::SUMS], fl
     Parts<T>::split_p(p, pf);
 }
 
-// ---- up to 16 query rows: a wave needs every K and V value once, so it loads them
-// from memory straight into the operands' layout (K: lane's key row, 8 elements a chunk;
-// V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
-// waves take every fourth step of the split and join at its end.
-constexpr int kFewWaves = 4, kFewUnit = kFewWaves * kStep;
-
 // Shares that follow each other run on one XCD (workgroups go round the XCDs): their
 // parts' row tiles, or beams' shared pages, are in one L2.
 __device__ __forceinline__ int share_id() {
@@ -519,28 +508,37 @@ __device__ __forceinline__ long out_row(const PagedArgs& a, const Span& sp, int 
     return ((long)sp.s * a.max_tok + rho / G) * a.n_heads + sp.kvh * G + rho % G;
 }
 
-template <int HD, class T>
-__global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) {
-    constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
-                  SUMS = Parts<T>::SUMS;
-    __shared__ float os[kFewWaves][16][HD + 4];
-    __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
+// The shares' loop of both kernels: `body` for each stretch of this workgroup's share.
+template <class Body>
+__device__ __forceinline__ void for_spans(const PagedArgs& a, int tile_rows, int unit, Body body) {
     __shared__ long cum[kPlanSeqs + 1], scan[4];
     __shared__ SeqLen lens[kPlanSeqs];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int n = lane & 15, g = lane >> 4, G = a.group;
-    make_plan(a, 16, kFewUnit, cum, scan, lens);
+    make_plan(a, tile_rows, unit, cum, scan, lens);
     if (blockIdx.x == 0)
-        for (int s = threadIdx.x; s <= a.n_seq; s += 256) a.plan[s] = cum[s];
+        for (int s = threadIdx.x; s <= a.n_seq; s += blockDim.x) a.plan[s] = cum[s];
     const long all = uniform(cum[a.n_seq]);
-    const int share = share_id();
-    const int used = shares_used(a, all);
+    const int share = share_id(), used = shares_used(a, all);
     if (share >= used) return;
     long lo = uniform(share_start(all, share, used));
     const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
-    while (lo < hi) {
-    const Span sp = next_span(a, cum, lens, 16, kFewUnit, share, seq, lo, hi);
+    while (lo < hi) body(next_span(a, cum, lens, tile_rows, unit, share, seq, lo, hi));
+}
+
+// ---- up to 16 query rows: a wave needs every K and V value once, so it loads them
+// from memory straight into the operands' layout (K: lane's key row, 8 elements a chunk;
+// V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
+// waves take every fourth step of the split and join at its end.
+constexpr int kFewWaves = 4, kFewUnit = kFewWaves * kStep;
+
+template <int HD, class T>
+__device__ __forceinline__ void few_span(const PagedArgs& a, const Span& sp) {
+    constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
+                  SUMS = Parts<T>::SUMS;
+    __shared__ float os[kFewWaves][16][HD + 4];
+    __shared__ float ms[kFewWaves][16], ls[kFewWaves][16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int n = lane & 15, g = lane >> 4, G = a.group;
     const int kvh = sp.kvh, tile = sp.tile, rows = sp.rows;
     const int rho = tile * 16 + n;
     const bool live = rho < rows;
@@ -712,7 +710,11 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
         }
     }
     __syncthreads();
-    }
+}
+
+template <int HD, class T>
+__global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) {
+    for_spans(a, 16, kFewUnit, [&](const Span& sp) { few_span<HD, T>(a, sp); });
 }
 
 // ---- more rows: the workgroup's NW waves share each step's K and V through LDS,
@@ -737,7 +739,7 @@ constexpr int many_bufs() {
 }
 
 template <int HD, class T, int NW, int MW>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
+__device__ __forceinline__ void many_span(const PagedArgs& a, const Span& sp) {
     constexpr int NC = HD / 32, ND = HD / 16, KP = Parts<T>::KP, QP = Parts<T>::QP,
                   SUMS = Parts<T>::SUMS, TR = 16 * NW * MW, NB = many_bufs<HD, T, NW>();
     // a thread's part of a step: EK times 8 elements of a key's K; EV elements of 8 keys' V.
@@ -749,22 +751,8 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
     __shared__ uint4 frag[NB][VL + ND * KP * 64];
     __shared__ uint64_t masks[TR];
     __shared__ uint32_t holes[NB];  // byte g, bit 4 tile + r: key 16 tile + 4 g + r is no row
-    __shared__ long cum[kPlanSeqs + 1], scan[4];
-    __shared__ SeqLen lens[kPlanSeqs];
     const int t = threadIdx.x, lane = t & 63, wave = __builtin_amdgcn_readfirstlane(t >> 6);
     const int n = lane & 15, g = lane >> 4, G = a.group;
-    make_plan(a, TR, kManyUnit, cum, scan, lens);
-    if (blockIdx.x == 0)
-        for (int s = t; s <= a.n_seq; s += 64 * NW) a.plan[s] = cum[s];
-    const long all = uniform(cum[a.n_seq]);
-    const int share = share_id();
-    const int used = shares_used(a, all);
-    if (share >= used) return;
-    long lo = uniform(share_start(all, share, used));
-    const long hi = uniform(share_start(all, share + 1, used));
-    int seq = 0;
-    while (lo < hi) {
-    const Span sp = next_span(a, cum, lens, TR, kManyUnit, share, seq, lo, hi);
     const int kvh = sp.kvh, rows = sp.rows, row0 = sp.tile * TR;
     const long ld = (long)a.n_kv_heads * HD;
 
@@ -895,8 +883,9 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
                 for (int tt = 0; tt < 2; tt++)
 #pragma unroll
                     for (int e = 0; e < SUMS; e++) st[w][tt][e] = f32x4{0.f, 0.f, 0.f, 0.f};
-            // fragments are read one product ahead of their use, and no further (the
-            // scheduling barriers: more of them in flight would not fit in registers)
+            // fragments are read one product ahead of their use, before that one's operands
+            // are waited for, and no further: the scheduling barriers (more of them in
+            // flight would not fit in registers)
             uint4 f[2][NA][KP];
             auto read_k = [&](int i) {  // product i: chunk i / (2 / NA), key tiles from i % (2 / NA) * NA
 #pragma unroll
@@ -910,6 +899,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
 #pragma unroll
             for (int i = 0; i < 2 * NC / NA; i++) {
                 if (i + 1 < 2 * NC / NA) read_k(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
                 const uint4* q[M];
                 f32x4* to[NA][M];
 #pragma unroll
@@ -948,6 +938,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
 #pragma unroll
             for (int i = 0; i < ND / NA; i++) {
                 if (i + 1 < ND / NA) read_v(i + 1);
+                __builtin_amdgcn_sched_barrier(0);
                 f32x4* to[NA][M];
 #pragma unroll
                 for (int x = 0; x < NA; x++)
@@ -991,7 +982,12 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
             *reinterpret_cast<f32x4_a4*>(dst + 16 * d + 4 * g) = y;
         }
     }
-    }
+}
+
+template <int HD, class T, int NW, int MW>
+__global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
+    for_spans(a, 16 * NW * MW, kManyUnit,
+              [&](const Span& sp) { many_span<HD, T, NW, MW>(a, sp); });
 }
 
 // One wave a query row and head.  Where its part lies in several shares, their sums are
