@@ -220,33 +220,35 @@ __device__ __forceinline__ void load8(const float* p, float (&v)[8]) {
     }
 }
 
-// q elements d .. d+7 (d % 8 == 0) of a row: bias and RoPE by the tables' row pos.
+// q elements d .. d+7 and HD/2 + d .. (d % 8 == 0, d < HD/2) of a row, which RoPE turns
+// into each other: bias and RoPE by the tables' row pos.
 template <int HD>
 __device__ __forceinline__ void q_values8(const PagedArgs& a, long row, int h, int d, long pos,
-                                          float (&x)[8]) {
-    const float* qr = a.q + row * a.q_ld + h * HD;
-    load8(qr + d, x);
-    float b[8];
+                                          float (&x)[8], float (&y)[8]) {
+    constexpr int half = HD / 2;
+    const float* qr = a.q + row * a.q_ld + h * HD + d;
+    load8(qr, x);
+    load8(qr + half, y);
     if (a.bq) {
+        float b[8], b2[8];
         load8(a.bq + h * HD + d, b);
+        load8(a.bq + h * HD + d + half, b2);
 #pragma unroll
-        for (int e = 0; e < 8; e++) x[e] += b[e];
+        for (int e = 0; e < 8; e++) {
+            x[e] += b[e];
+            y[e] += b2[e];
+        }
     }
     if (a.pos) {
-        constexpr int half = HD / 2;
-        const int e2 = d < half ? d + half : d - half, f = d < half ? d : e2;
-        float y[8], c[8], s[8];
-        load8(qr + e2, y);
-        load8(a.cos_t + pos * half + f, c);
-        load8(a.sin_t + pos * half + f, s);
-        if (a.bq) {
-            load8(a.bq + h * HD + e2, b);
+        float c[8], s[8];
+        load8(a.cos_t + pos * half + d, c);
+        load8(a.sin_t + pos * half + d, s);
 #pragma unroll
-            for (int e = 0; e < 8; e++) y[e] += b[e];
+        for (int e = 0; e < 8; e++) {
+            const float u = x[e], w = y[e];
+            x[e] = fmaf(u, c[e], -(w * s[e]));
+            y[e] = fmaf(w, c[e], u * s[e]);
         }
-        const float sign = d < half ? -1.f : 1.f;
-#pragma unroll
-        for (int e = 0; e < 8; e++) x[e] = fmaf(x[e], c[e], sign * (y[e] * s[e]));
     }
 }
 // The row's position in the RoPE tables.
@@ -263,10 +265,16 @@ __device__ __forceinline__ long q_pos(const PagedArgs& a, long row) {
 // k_attn_paged_join adds.
 constexpr int kPlanSeqs = 256;  // sequences a launch
 
-// a / b of whole numbers, a >= 0, b > 0, a / b < 2^51 (no 64-bit integer division in
-// hardware): the rounded quotient is off by one at the most.
+// a / b of whole numbers, a >= 0, b > 0, a / b < 2^50: hardware has no 64-bit integer
+// division, and a correctly rounded one in doubles is 35 instructions.  1 / b from the
+// approximation (2^-23 or better) in two Newton steps is good to 2^-51, so the product's
+// whole part is off by one at the most.
 __device__ __forceinline__ long div_whole(long a, long b) {
-    long q = (long)((double)a / (double)b);
+    const double d = (double)b;
+    double y = __builtin_amdgcn_rcp(d);
+    y = fma(fma(-d, y, 1.), y, y);
+    y = fma(fma(-d, y, 1.), y, y);
+    const long q = (long)((double)a * y);
     const long r = a - q * b;
     return r < 0 ? q - 1 : (r >= b ? q + 1 : q);
 }
@@ -340,7 +348,13 @@ struct Span {
 __device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, const SeqLen* lens,
                                           int tile_rows, int unit, int share, int& s, long& lo,
                                           long hi) {
-    while (lo >= uniform(cum[s + 1])) s++;
+    // sequences whose units end at lo or before, 64 at a time
+    for (;;) {
+        const int t = s + (threadIdx.x & 63);
+        const int n = __popcll(__ballot(t < a.n_seq && cum[t + 1] <= lo));
+        s += n;
+        if (n < 64) break;
+    }
     Span p;
     p.s = s;
     SeqLen n = lens[s];
@@ -431,8 +445,8 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int r
     const int g = (threadIdx.x & 63) >> 4, i = rho / a.group, h = sp.kvh * a.group + rho - i * a.group;
     float x[NC][8];
 #pragma unroll
-    for (int c = 0; c < NC; c++)
-        q_values8<HD>(a, (long)sp.s * a.max_tok + i, h, 32 * c + 8 * g, pos, x[c]);
+    for (int c = 0; c < NC / 2; c++)
+        q_values8<HD>(a, (long)sp.s * a.max_tok + i, h, 32 * c + 8 * g, pos, x[c], x[c + NC / 2]);
     constexpr float kRoot = HD == 64 ? 8.f : HD == 256 ? 16.f : 11.3137084989847603904f;
     scale = kLog2e / kRoot;
     float up = 1.f;
@@ -471,10 +485,10 @@ __device__ __forceinline__ void weights(const f32x4 (&st)[2][Parts<T>::SUMS], fl
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const int j = jb + 16 * (e >> 2) + 4 * g + (e & 3);
-            const bool own = j >= sp.held;
-            const bool see = j < sp.j1 && !((bad >> e) & 1) &&
-                             (!own || ((mask >> (own ? j - sp.held : 0)) & 1));
-            s[e] = see ? s[e] : -INFINITY;
+            // without branches; a key that the cache held is seen by all
+            const uint32_t own = j >= sp.held ? (uint32_t)(mask >> ((j - sp.held) & 63)) : 1u;
+            const uint32_t see = own & ~(bad >> e) & (uint32_t)(j < sp.j1);
+            s[e] = see & 1 ? s[e] : -INFINITY;
         }
     }
     float top = s[0];
