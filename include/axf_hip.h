@@ -292,8 +292,9 @@ int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n)
  *   - parent[i] outside 0..n_in-1 or len[i] < 0: sequence i holds nothing.
  * A text starts as an input row of -1 with len 0.  table_out: n_out rows of
  * table_ld entries, entries past the room -1, not the array `table`.  refs_out
- * (n_pages) may be refs; refs has to count what the tables hold.  info (3 int32): copied pages, entries left without a
- * page, pages free afterwards.  Room past table_ld pages is cut off there. */
+ * (n_pages) may be refs; refs has to count what the tables hold.  info (3 int32):
+ * copied pages, entries left without a page, pages free afterwards.  Room past
+ * table_ld pages is cut off there. */
 int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, int32_t* refs_out,
                     int32_t* info, const int32_t* table, const int32_t* refs, int n_in,
                     const int32_t* parent, const int32_t* len, int n_out, int table_ld, int extra);

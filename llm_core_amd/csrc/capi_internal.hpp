@@ -340,6 +340,7 @@ struct PagedArgs {
     float* out;
     uint8_t* outq8;
     int shares;       // workgroups that the keys are dealt out to (attn_paged_plan)
+    int per;          // steps of 32 keys a unit of the dealing (attn_paged_plan)
     // set by the launcher, in its scratch
     float* part;      // [share][2][tile rows][HD]: unfinished weighted V sums
     float2* part_ml;  // [share][2][tile rows]: their maximum (base 2) and weight sum

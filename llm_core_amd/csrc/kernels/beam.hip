@@ -12,6 +12,9 @@
 //   2. k_beam_merge: a workgroup a sequence joins the chunks' sums to each beam's
 //      lse, turns the keys into scores and picks the n_out best of the chunks' sorted
 //      lists.
+// 8 x 8 beams of 151936 (38.9 MB, 7.5 us at a large copy's rate): 17.6 + 10.2 us; the
+// first is bound by the 64-bit arithmetic (9.7 million logits at about 20 operations), the
+// second by the latencies of one workgroup a sequence.  1 x 4 of 32000: 4.1 + 5.6 us.
 #include "common.hpp"
 
 namespace axf {

@@ -257,7 +257,7 @@ __device__ __forceinline__ long q_pos(const PagedArgs& a, long row) {
 }
 
 // How the work is split.  A part is one sequence's, KV head's and row tile's walk over
-// its keys, in units of `unit` keys; all parts' units in a row are dealt out evenly to
+// its keys, in units of `per` steps; all parts' units in a row are dealt out evenly to
 // the grid's workgroups, which are as many as run at once: every workgroup has the same
 // number of units, however ragged the lengths, and a part that lies in one share is
 // finished there.  A share holds at most two unfinished ends (its first part's and its
@@ -279,30 +279,42 @@ __device__ __forceinline__ long div_whole(long a, long b) {
     return r < 0 ? q - 1 : (r >= b ? q + 1 : q);
 }
 
+// A unit is `per` steps of 32 keys.  With per 3 a last tile at most half full has units of
+// 4 steps: its waves without rows leave the others the SIMDs, and a step takes 0.74 of a
+// full tile's time (16 sequences @8000, 64 and 128 rows: 275 and 368 us).  48 tokens (192
+// rows): 593 us, with units of 3 steps for both 618, of 1 618.
 struct SeqWork {
-    int rows, tiles;
-    long units;  // of one part
+    int rows, tiles, per_last;
+    long units, last;  // of a part, of one of the last row tile
+    __device__ __forceinline__ long of_head() const { return (tiles - 1) * units + last; }
 };
-// tile_rows and unit are powers of two
-__device__ __forceinline__ SeqWork seq_work(const SeqLen& n, int G, int tile_rows, int unit) {
+__device__ __forceinline__ long units_of(uint32_t steps, int per) {
+    return per == 3 ? (steps + 2) / 3 : (steps + per - 1) >> __builtin_ctz(per);
+}
+// tile_rows is a power of two
+__device__ __forceinline__ SeqWork seq_work(const SeqLen& n, int G, int tile_rows, int per) {
     SeqWork w;
     w.rows = n.tok * G;
     w.tiles = (w.rows + tile_rows - 1) >> __builtin_ctz(tile_rows);
-    w.units = w.tiles ? ((long)n.held + n.tok + unit - 1) >> __builtin_ctz(unit) : 0;
+    const int over = w.rows & (tile_rows - 1);
+    w.per_last = per == 3 && over && over <= tile_rows / 2 ? 4 : per;
+    const uint32_t steps = ((uint32_t)n.held + n.tok + kStep - 1) / kStep;
+    w.units = w.tiles ? units_of(steps, per) : 0;
+    w.last = w.tiles ? units_of(steps, w.per_last) : 0;
     return w;
 }
 
 // cum[s]: units before sequence s (cum[n_seq]: all), and its lengths; the first 256
 // threads.
-__device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, int unit, long* cum,
+__device__ __forceinline__ void make_plan(const PagedArgs& a, int tile_rows, long* cum,
                                           long* part, SeqLen* lens) {
     const int t = threadIdx.x, lane = t & 63;
     long w = 0;
     if (t < a.n_seq) {
         const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, t, a.table_ld, a.page_shift);
         lens[t] = n;
-        const SeqWork k = seq_work(n, a.group, tile_rows, unit);
-        w = k.units * k.tiles * a.n_kv_heads;
+        const SeqWork k = seq_work(n, a.group, tile_rows, a.per);
+        w = k.of_head() * a.n_kv_heads;
     }
 #pragma unroll
     for (int off = 1; off < 64; off <<= 1) {
@@ -346,8 +358,7 @@ struct Span {
 
 // The stretch at unit lo of a share that ends at hi; moves lo behind it.
 __device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, const SeqLen* lens,
-                                          int tile_rows, int unit, int share, int& s, long& lo,
-                                          long hi) {
+                                          int tile_rows, int share, int& s, long& lo, long hi) {
     // sequences whose units end at lo or before, 64 at a time
     for (;;) {
         const int t = s + (threadIdx.x & 63);
@@ -360,18 +371,22 @@ __device__ __forceinline__ Span next_span(const PagedArgs& a, const long* cum, c
     SeqLen n = lens[s];
     n.held = __builtin_amdgcn_readfirstlane(n.held);
     n.tok = __builtin_amdgcn_readfirstlane(n.tok);
-    const SeqWork w = seq_work(n, a.group, tile_rows, unit);
+    const SeqWork w = seq_work(n, a.group, tile_rows, a.per);
     p.held = n.held;
     p.tok = n.tok;
     p.rows = w.rows;
     p.table = a.table + (long)p.s * a.table_ld;
-    const long at = lo - uniform(cum[p.s]), part = uniform(div_whole(at, w.units));
-    const long u0 = at - part * w.units, u1 = min(w.units, u0 + hi - lo);
-    p.kvh = __builtin_amdgcn_readfirstlane((int)((uint32_t)part / (uint32_t)w.tiles));
-    p.tile = (int)part - p.kvh * w.tiles;
-    p.j0 = __builtin_amdgcn_readfirstlane((int)(u0 * unit));
-    p.j1 = __builtin_amdgcn_readfirstlane((int)min(u1 * unit, (long)n.held + n.tok));
-    p.slot = u0 > 0 ? 2 * share : (u1 < w.units ? 2 * share + 1 : -1);
+    const long at = lo - uniform(cum[p.s]), head = uniform(div_whole(at, w.of_head()));
+    const long in = at - head * w.of_head();
+    p.kvh = (int)head;
+    p.tile = w.tiles > 1 ? min((int)uniform(div_whole(in, w.units)), w.tiles - 1) : 0;
+    const bool end = p.tile == w.tiles - 1;
+    const long n_units = end ? w.last : w.units;
+    const int keys = (end ? w.per_last : a.per) * kStep;  // of a unit
+    const long u0 = in - p.tile * w.units, u1 = min(n_units, u0 + hi - lo);
+    p.j0 = __builtin_amdgcn_readfirstlane((int)(u0 * keys));
+    p.j1 = __builtin_amdgcn_readfirstlane((int)min(u1 * keys, (long)n.held + n.tok));
+    p.slot = u0 > 0 ? 2 * share : (u1 < n_units ? 2 * share + 1 : -1);
     lo += u1 - u0;
     return p;
 }
@@ -524,10 +539,10 @@ __device__ __forceinline__ long out_row(const PagedArgs& a, const Span& sp, int 
 
 // The shares' loop of both kernels: `body` for each stretch of this workgroup's share.
 template <class Body>
-__device__ __forceinline__ void for_spans(const PagedArgs& a, int tile_rows, int unit, Body body) {
+__device__ __forceinline__ void for_spans(const PagedArgs& a, int tile_rows, Body body) {
     __shared__ long cum[kPlanSeqs + 1], scan[4];
     __shared__ SeqLen lens[kPlanSeqs];
-    make_plan(a, tile_rows, unit, cum, scan, lens);
+    make_plan(a, tile_rows, cum, scan, lens);
     if (blockIdx.x == 0)
         for (int s = threadIdx.x; s <= a.n_seq; s += blockDim.x) a.plan[s] = cum[s];
     const long all = uniform(cum[a.n_seq]);
@@ -536,14 +551,21 @@ __device__ __forceinline__ void for_spans(const PagedArgs& a, int tile_rows, int
     long lo = uniform(share_start(all, share, used));
     const long hi = uniform(share_start(all, share + 1, used));
     int seq = 0;
-    while (lo < hi) body(next_span(a, cum, lens, tile_rows, unit, share, seq, lo, hi));
+    while (lo < hi) body(next_span(a, cum, lens, tile_rows, share, seq, lo, hi));
 }
 
 // ---- up to 16 query rows: a wave needs every K and V value once, so it loads them
 // from memory straight into the operands' layout (K: lane's key row, 8 elements a chunk;
 // V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
 // waves take every fourth step of the split and join at its end.
-constexpr int kFewWaves = 4, kFewUnit = kFewWaves * kStep;
+//
+// Bound by HBM where the cache is long: 16 sequences @4000 of 32/8 heads of 128, one token:
+// F32 71.6 us (4.6 TB/s), F16 43.0 (3.8 TB/s; half the bytes for the same steps).  One
+// token @1024 (24 workgroups) is a chain of latencies, 11.5 us + 3.9 of the join: 1.6 to
+// start, 1 for the lengths' plan, 1.2 for the span, 2.6 and 1.9 for the table's and then
+// K's and q's loads, 3.1 for the step's arithmetic (splits, products and softmax of one
+// wave a SIMD), 1.1 to join the waves.
+constexpr int kFewWaves = 4;
 
 template <int HD, class T>
 __device__ __forceinline__ void few_span(const PagedArgs& a, const Span& sp) {
@@ -728,7 +750,7 @@ __device__ __forceinline__ void few_span(const PagedArgs& a, const Span& sp) {
 
 template <int HD, class T>
 __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) {
-    for_spans(a, 16, kFewUnit, [&](const Span& sp) { few_span<HD, T>(a, sp); });
+    for_spans(a, 16, [&](const Span& sp) { few_span<HD, T>(a, sp); });
 }
 
 // ---- more rows: the workgroup's NW waves share each step's K and V through LDS,
@@ -739,7 +761,15 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
 // beside its products is the cache read again, so a tile is as large as registers allow:
 // 64 rows of 4 waves, two workgroups a CU, else 128 or 256 of 8 waves.  The next step's
 // values are in flight while this one is multiplied.
-constexpr int kManyUnit = kStep;
+//
+// 16 trees of up to 48 tokens, 32/8 heads of 128 @8191, F32: 382 us, 128 TFLOP/s of scores
+// and sums where six bf16 products a value allow 200 at a large library product's rate
+// (243 us).  What bounds it is no one unit; of 402 us before its last steps, with half the
+// products 307, without the splitting 371, with a third of the LDS reads 375, without
+// loads 360, loads and splitting alone 231.  The two waves of a SIMD go through the step's phases together,
+// between the same barriers.  Tried: K of the next step multiplied under this one's
+// softmax (427), one LDS buffer and 2 workgroups (419), raised priority around the
+// products (400), 4 waves of three tiles (158 registers spilt, 822).
 
 // LDS of one step's fragments, and how many steps' fit beside each other (two: one
 // barrier a step instead of two) with the workgroups a CU is to hold.
@@ -1000,16 +1030,17 @@ __device__ __forceinline__ void many_span(const PagedArgs& a, const Span& sp) {
 
 template <int HD, class T, int NW, int MW>
 __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
-    for_spans(a, 16 * NW * MW, kManyUnit,
-              [&](const Span& sp) { many_span<HD, T, NW, MW>(a, sp); });
+    for_spans(a, 16 * NW * MW, [&](const Span& sp) { many_span<HD, T, NW, MW>(a, sp); });
 }
 
 // One wave a query row and head.  Where its part lies in several shares, their sums are
 // brought to one base and added in their order, and divided by the weights' sum (lane j
 // has share j's m and l, so one load's latency covers 64 of them); a whole part's row
-// is read back.  A row that is not finite is done again with care.
+// is read back.  A row that is not finite is done again with care.  3.9 us for 16 rows, 4.1
+// for 672 (launch and three loads after each other: plan, m and l, sums); 15.6 us for
+// 24576 rows of 128 whose 256 shares' sums are 34 MB.
 template <int HD, class T>
-__global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows, int unit) {
+__global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows) {
     constexpr int E = HD / 64, U = 8;
     const int lane = threadIdx.x & 63;
     const uint32_t w = __builtin_amdgcn_readfirstlane(blockIdx.x * 4 + (threadIdx.x >> 6));
@@ -1020,13 +1051,14 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
     const long all = a.plan[a.n_seq], before = a.plan[s];
     const SeqLen n = seq_len(a.len, a.n_tok, a.max_tok, s, a.table_ld, a.page_shift);
     if (i >= n.tok) return;
-    const SeqWork sw = seq_work(n, G, tile_rows, unit);
+    const SeqWork sw = seq_work(n, G, tile_rows, a.per);
     const int kvh = (int)((uint32_t)h / (uint32_t)G), rho = i * G + h - kvh * G;
     const int tile = rho >> __builtin_ctz(tile_rows);
-    const long p0 = before + ((long)kvh * sw.tiles + tile) * sw.units;
+    const long p0 = before + kvh * sw.of_head() + tile * sw.units;
+    const long p1 = p0 + (tile == sw.tiles - 1 ? sw.last : sw.units) - 1;
     const int shares = shares_used(a, all);
     const int w1 = __builtin_amdgcn_readfirstlane(share_of(all, p0, shares));
-    const int w2 = __builtin_amdgcn_readfirstlane(share_of(all, p0 + sw.units - 1, shares));
+    const int w2 = __builtin_amdgcn_readfirstlane(share_of(all, p1, shares));
     float* dst = a.out + (long)w * HD + lane * E;
     float o[E], l = 1.f;
     if (w1 == w2) {
@@ -1105,7 +1137,9 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
 
 // ---- store -----------------------------------------------------------------
 // One thread 4 + 4 values of K (a RoPE pair's halves) and of V: element d..d+3 and
-// d+HD/2.. of one head.  Bandwidth: each value is read and written once.
+// d+HD/2.. of one head.  Each value is read and written once: 24 sequences of 48 tokens,
+// 8 heads of 128, F16 (14.1 MB) 4.3 us, 3.3 TB/s; 8 rows of 2 heads of 128 3.0 us, a
+// launch's time.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
     constexpr int PER = HD / 8;  // threads a head
@@ -1159,7 +1193,8 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
 // barriers between its steps and no other launch.  Reference counts are atomics (whole
 // numbers, so their order does not matter), in LDS up to kForkLdsPages pages: one CU's
 // scattered atomics to L2 go one a cycle or less, 128 sequences of 49 pages took 19 us
-// with them.  Everything else goes by index order.
+// with them.  Everything else goes by index order.  4 beams @1000 5.5 us, 16 x 8 @1500
+// 11: the walk's steps after each other, each a load's or a scan's latency.
 constexpr int kForkThreads = 1024;
 constexpr int kForkLdsPages = 32768;  // 128 KiB
 
@@ -1374,6 +1409,8 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
 }
 
 // The copied pages' rows: workgroup (output, layer and K or V, 16 KiB of the page).
+// 128 pages' rows in 24 layers, 12.6 MB read and written again: 4.7 to 6.6 us, 3.8 TB/s
+// and up; 1.8 to 2.4 us where little is copied.
 constexpr int kCopyBytes = 16384;
 
 __global__ __launch_bounds__(256) void k_kv_copy(uint8_t* k, uint8_t* v, const int* copy,
@@ -1404,6 +1441,8 @@ __device__ __forceinline__ int path_length(const int* way, int most) {
 // Workgroup (sequence, layer, K or V): each thread owns 16-byte columns and moves rows in
 // path order, eight reads at a time.  path[i] >= i and ascending: a row is written
 // only after every read of it (an earlier write goes to a lower row than every later read).
+// 16 trees of 32 nodes in 32 layers of 4 KiB rows, 80 MB: 15.8 to 18 us, 4.4 to 5.1 TB/s,
+// what a large copy reaches; one tree of 16 in 2 layers 2.4 to 3 us, a launch's time.
 __global__ __launch_bounds__(256) void k_kv_compact(uint8_t* k, uint8_t* v, int* len_out,
                                                     const int* table, int table_ld,
                                                     const int* len, const int* path,
@@ -1453,15 +1492,18 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
     if ((threadIdx.x & 63) == 0) len_out[s] = kv_len(len[s], table_ld, page_shift) + n;
 }
 
-// Query rows of a KV head that a workgroup takes: the fewest that hold them all, so that
-// the cache is read once, as far as two tiles' operands and sums fit in a wave's 256
-// registers: at 64 elements a head, and at 128 with F16 pages' two parts of q.  (F32 at
-// 128: 40 registers spilt, 16 trees of 48 tokens @8191 in 446 us against 402 with
-// 128-row tiles that read the cache twice.)
+// Query rows of a KV head that a workgroup takes: the fewest that hold them all, up to
+// 128.  Measured against the next larger tile: 16 sequences @4000 of 32/8 heads of 128, F32,
+// one token (4 rows): 71.6 us, 64-row tiles 78.8; 12 tokens (48 rows): 93.3 us, 128-row
+// tiles 103.6.  256 rows (two tiles a wave, each fragment read from LDS once for both; the
+// cache read once for them, which L2 gives to 128-row tiles too) pay where the products are
+// the least of a step, 64 elements a head with F16 pages: 16 trees of 48 tokens, 28/4
+// heads @8000: 169.7 us, 128-row tiles 184.1; F16 at 128 elements 191.7 and 190.0, F32 at
+// 64 208.7 and 210.2; F32 at 128, 16 trees @8191 (40 registers spilt) 446 and 402.
 int tile_rows(int rows, int head_dim, int kv_type) {
     if (rows <= 16) return 16;
     if (rows <= 64) return 64;
-    return rows > 128 && (head_dim == 64 || (head_dim == 128 && kv_type == AXF_TYPE_F16)) ? 256 : 128;
+    return rows > 128 && head_dim == 64 && kv_type == AXF_TYPE_F16 ? 256 : 128;
 }
 
 template <int HD, class T>
@@ -1475,12 +1517,11 @@ hipError_t attn_launch(const PagedArgs& a, hipStream_t st) {
     } else if (tr == 128) {
         k_attn_paged_many<HD, T, 8, 1><<<a.shares, 512, 0, st>>>(a);
     } else {
-        if constexpr (HD == 64 || (HD == 128 && sizeof(T) == 2))
+        if constexpr (HD == 64 && sizeof(T) == 2)
             k_attn_paged_many<HD, T, 8, 2><<<a.shares, 512, 0, st>>>(a);
     }
     const long waves = (long)a.n_seq * a.max_tok * a.n_heads;
-    k_attn_paged_join<HD, T><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(
-        a, tr, tr == 16 ? kFewUnit : kManyUnit);
+    k_attn_paged_join<HD, T><<<(unsigned)((waves + 3) / 4), 256, 0, st>>>(a, tr);
     return hipGetLastError();
 }
 
@@ -1515,8 +1556,9 @@ void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
     const int rows = a.max_tok * a.group, tr = tile_rows(rows, head_dim, kv_type);
     const long seqs = a.n_seq < kPlanSeqs ? a.n_seq : kPlanSeqs;
-    const long units = (longest + (tr == 16 ? kFewUnit : kManyUnit) - 1) /
-                       (tr == 16 ? kFewUnit : kManyUnit) * seqs * a.n_kv_heads * ((rows + tr - 1) / tr);
+    a.per = tr == 16 ? kFewWaves : (tr == 128 && rows > 128 ? 3 : 1);
+    const long units = (longest + a.per * kStep - 1) / (a.per * kStep) * seqs * a.n_kv_heads *
+                       ((rows + tr - 1) / tr);
     const long most = tr == 64 || (tr == 16 && head_dim == 64) ? 512 : 256;
     const long shares = units < most ? units : most;
     a.shares = (int)((shares + 7) & ~7L);
