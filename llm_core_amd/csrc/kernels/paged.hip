@@ -762,7 +762,7 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
 // 64 rows of 4 waves, two workgroups a CU, else 128 or 256 of 8 waves.  The next step's
 // values are in flight while this one is multiplied.
 //
-// 16 trees of up to 48 tokens, 32/8 heads of 128 @8191, F32: 382 us, 128 TFLOP/s of scores
+// 16 trees of up to 48 tokens, 32/8 heads of 128 @8191, F32: 380 us, 129 TFLOP/s of scores
 // and sums where six bf16 products a value allow 200 at a large library product's rate
 // (243 us).  What bounds it is no one unit; of 402 us before its last steps, with half the
 // products 307, without the splitting 371, with a third of the LDS reads 375, without
@@ -1037,7 +1037,7 @@ __global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
 // brought to one base and added in their order, and divided by the weights' sum (lane j
 // has share j's m and l, so one load's latency covers 64 of them); a whole part's row
 // is read back.  A row that is not finite is done again with care.  3.9 us for 16 rows, 4.1
-// for 672 (launch and three loads after each other: plan, m and l, sums); 15.6 us for
+// for 672 (launch and three loads after each other: plan, m and l, sums); 16.3 us for
 // 24576 rows of 128 whose 256 shares' sums are 34 MB.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows) {
@@ -1194,7 +1194,7 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
 // numbers, so their order does not matter), in LDS up to kForkLdsPages pages: one CU's
 // scattered atomics to L2 go one a cycle or less, 128 sequences of 49 pages took 19 us
 // with them.  Everything else goes by index order.  4 beams @1000 5.5 us, 16 x 8 @1500
-// 11: the walk's steps after each other, each a load's or a scan's latency.
+// 8.7: the walk's steps after each other, each a load's or a scan's latency.
 constexpr int kForkThreads = 1024;
 constexpr int kForkLdsPages = 32768;  // 128 KiB
 
@@ -1409,8 +1409,8 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
 }
 
 // The copied pages' rows: workgroup (output, layer and K or V, 16 KiB of the page).
-// 128 pages' rows in 24 layers, 12.6 MB read and written again: 4.7 to 6.6 us, 3.8 TB/s
-// and up; 1.8 to 2.4 us where little is copied.
+// 128 pages' rows in 24 layers, 12.6 MB read and written again: 5.1 to 6.6 us, 3.8 to 4.9
+// TB/s; 1.8 to 2.4 us where little is copied.
 constexpr int kCopyBytes = 16384;
 
 __global__ __launch_bounds__(256) void k_kv_copy(uint8_t* k, uint8_t* v, const int* copy,
