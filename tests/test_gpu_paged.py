@@ -141,6 +141,19 @@ def test_attn_long(ctx, tok, kv, hd):
         c.check(c.run(ctx, max_len=max_len), *want)
 
 
+@pytest.mark.parametrize("heads,kvh,hd,tok,kv", [
+    (32, 8, 128, 48, "f32"), (16, 2, 64, 40, "f32"), (24, 4, 128, 43, "f16"),
+    (8, 2, 256, 37, "f32"), (28, 4, 64, 64, "f16"), (32, 4, 128, 64, "f32")])
+def test_attn_row_tiles(ctx, heads, kvh, hd, tok, kv):
+    """Rows that fill their last tile by a little, by half, more and in full, in sequences
+    of one call, with their keys split over many workgroups and over few."""
+    c = Case(heads + tok, heads, kvh, hd, kv, 16, [2003, 701, 0, 95], [tok, tok - 17, 1, tok], tok,
+             mask="tree")
+    want = c.want()
+    for max_len in (2003, 0):
+        c.check(c.run(ctx, max_len=max_len), *want)
+
+
 @pytest.mark.parametrize("tok", [1, 20])
 def test_attn_q8(ctx, tok):
     """outq8 holds the Q8_0 blocks of out, bit for bit; rows past n_tok stay."""
