@@ -1029,7 +1029,8 @@ __device__ __forceinline__ void many_span(const PagedArgs& a, const Span& sp) {
 }
 
 template <int HD, class T, int NW, int MW>
-__global__ __launch_bounds__(64 * NW, 2) void k_attn_paged_many(PagedArgs a) {
+__global__ __launch_bounds__(64 * NW, NW == 4 && HD == 256 && sizeof(T) == 4 ? 1 : 2)
+void k_attn_paged_many(PagedArgs a) {
     for_spans(a, 16 * NW * MW, [&](const Span& sp) { many_span<HD, T, NW, MW>(a, sp); });
 }
 
@@ -1546,11 +1547,11 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 }  // namespace
 
 // Workgroups of the launch: as many as run at once, or as few as have a unit each by the
-// caller's estimate of the lengths.  A CU holds two workgroups of 64-row tiles, or of few
-// rows at 64 elements a head (fewer than 256 registers); one of few rows at 128 and 256
-// elements, or of 8 waves.  More than run at once leave the last ones a CU to
+// caller's estimate of the lengths.  A CU holds two workgroups of 64-row tiles (with F32 at
+// 256 elements one: LDS), or of few rows at 64 elements a head (fewer than 256 registers);
+// one of few rows at 128 and 256 elements, or of 8 waves.  More than run at once leave the last ones a CU to
 // themselves: 16 sequences of 32/8 heads @4000 with 256, 512, 1024 workgroups: 73, 83,
-// 98 us.
+// 98 us; 12 tokens each, 16/4 heads of 256, F32 (96 KiB of LDS) with 256 and 512: 134, 146.
 void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;
@@ -1559,7 +1560,8 @@ void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     a.per = tr == 16 ? kFewWaves : (tr == 128 && rows > 128 ? 3 : 1);
     const long units = (longest + a.per * kStep - 1) / (a.per * kStep) * seqs * a.n_kv_heads *
                        ((rows + tr - 1) / tr);
-    const long most = tr == 64 || (tr == 16 && head_dim == 64) ? 512 : 256;
+    const bool alone = head_dim == 256 && kv_type == AXF_TYPE_F32;
+    const long most = (tr == 64 && !alone) || (tr == 16 && head_dim == 64) ? 512 : 256;
     const long shares = units < most ? units : most;
     a.shares = (int)((shares + 7) & ~7L);
 }

@@ -73,6 +73,19 @@ def test_select(ctx, V, kind):
         check(got, x, cum, done, eos, n_out)
 
 
+@pytest.mark.parametrize("kind", ["normal", "ascending", "equal", "masked"])
+@pytest.mark.parametrize("n,B,V,n_out", [(2, 16, 8000, 32), (4, 16, 60000, 32), (3, 20, 4099, 40),
+                                         (1, 33, 9001, 33), (2, 64, 2500, 64), (1, 64, 17001, 63)])
+def test_select_many_kept(ctx, n, B, V, n_out, kind):
+    """n_out no small part of a wave: bounds by 64 lists leave more than can be ranked."""
+    rng = np.random.default_rng(n_out + V)
+    x = logits_of(kind, (n, B, V), rng)
+    for spread in (0.5, 40.0):
+        cum = (-spread * rng.random((n, B))).astype(np.float32)
+        done = (rng.random((n, B)) < 0.2).astype(np.int32)
+        check(run(ctx, x, cum, done, 5, n_out), x, cum, done, 5, n_out)
+
+
 @pytest.mark.parametrize("n,B,V,n_out", [(2, 8, 151936, 16), (1, 64, 32000, 64), (40, 2, 4099, 4),
                                          (1, 1, 300001, 64)])
 def test_select_large(ctx, n, B, V, n_out):
