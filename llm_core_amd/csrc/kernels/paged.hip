@@ -60,9 +60,12 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
 //   h + 2^-12 l, two fp16 parts with a sum of their own each, 22 bits of every element;
 //   p (times 2^15) is h + l with one sum, 22 bits down to p = 2^-16 and 2^-39 below
 //   (a second sum would cost O's registers again): two products, no work on K or V.
+//   A subnormal value (below 2^-14) counts with the exponent -14 where products are
+//   aligned, so what is below 2^-37 of O (2^-23 of that exponent) is cut off there.
 // Infinities and NaN do not split, and 0 times one of them in a masked place is NaN: a
 // row whose result is not finite is done again in plain fp32 (row_careful, by the
-// joining kernel), where masked places are left out.
+// joining kernel), where masked places are left out.  So is a row whose scores are too
+// far out (far_out), whose result is made NaN.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -193,6 +196,15 @@ struct Parts<_Float16> {
         return fmaf(c[1][r], 1.f / 4096.f, c[0][r]);
     }
 };
+
+// A weight is exp2(s c - m), its product not rounded but m, the largest one, rounded to
+// fp32: all of a row's weights are too large or small by one factor, 2^(half a step of m)
+// at the most, which their sum takes out again.  Up to |m| = 2^22 it is 2^0.25; from 2^28
+// on it leaves fp16 parts without digits, from 2^31 on weights without any.  top: the row's
+// largest score (base 2), -inf where it sees nothing.
+__device__ __forceinline__ bool far_out(float top) {
+    return fabsf(top) > 4194304.f && top != -INFINITY;
+}
 
 // Reductions over the four 16-lane rows of a wave (lanes n, n + 16, n + 32, n + 48),
 // every lane receiving the result.  v_permlane{16,32}_swap of a value with itself
@@ -732,7 +744,7 @@ __device__ __forceinline__ void few_span(const PagedArgs& a, const Span& sp) {
             dst = a.part + ((long)sp.slot * 16 + t) * HD;
             if (u == 0) a.part_ml[sp.slot * 16 + t] = make_float2(top, sum);
         }
-        const float by = !whole ? 1.f : (sum == 0.f ? 0.f : 1.f / sum);
+        const float by = !whole ? 1.f : far_out(top) ? NAN : (sum == 0.f ? 0.f : 1.f / sum);
         for (int d = 4 * u; d < HD; d += 64) {
             float y[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -1017,7 +1029,8 @@ __device__ __forceinline__ void many_span(const PagedArgs& a, const Span& sp) {
         float* dst = whole ? a.out + out_row(a, sp, row0 + in + n) * HD
                            : a.part + ((long)sp.slot * TR + in + n) * HD;
         if (!whole && g == 0) a.part_ml[sp.slot * TR + in + n] = make_float2(m[w], l[w]);
-        const float by = (!whole ? 1.f : (l[w] == 0.f ? 0.f : 1.f / l[w])) / Parts<T>::kUp;
+        const float by =
+            (!whole ? 1.f : far_out(m[w]) ? NAN : (l[w] == 0.f ? 0.f : 1.f / l[w])) / Parts<T>::kUp;
 #pragma unroll
         for (int d = 0; d < ND; d++) {
             f32x4_a4 y;
@@ -1105,7 +1118,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
                 }
             }
         }
-        const float by = l == 0.f ? 0.f : 1.f / l;
+        const float by = far_out(top) ? NAN : (l == 0.f ? 0.f : 1.f / l);
 #pragma unroll
         for (int e = 0; e < E; e++) o[e] *= by;
     }
