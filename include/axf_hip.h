@@ -324,7 +324,10 @@ int axf_hip_kv_store(axf_ctx* ctx, const axf_kv_pages* kv, int layer, const int3
  * (NaN and infinities too) changes nothing; a score of -inf has no weight, one of
  * +inf or NaN makes its row NaN.  out is apart from q.  max_len: about the longest
  * len[s], for the split of the work; any value gives the same sums up to their
- * order.  Held in fp32 throughout. */
+ * order.  Precision: sums, maxima and results are fp32.  F32 pages: products to 2^-21, as
+ * a rule 2^-24, of themselves; rows that values below 2^-110 or scores past 2^22 would show in
+ * are computed in plain fp32, slowly.  F16 pages: K and V as stored, q and the weights
+ * in 22 bits. */
 int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, int q_ld,
                        const float* bq, const axf_kv_pages* kv, int layer, const int32_t* table,
                        int table_ld, const int32_t* len, const int32_t* n_tok,

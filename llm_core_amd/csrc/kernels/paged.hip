@@ -53,9 +53,10 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
 // exchange either.
 //
 // fp32 is kept on 16-bit operands by splitting:
-//   F32 pages: x = h + m + l, three bf16 cut off one after the other (exact: 8 bits
-//   each, the whole range of fp32, no scales), and the six products that reach 2^-24
-//   of the largest: hh, hm, mh, mm, hl, lh; 6/16 of the fp32 matrix rate's time.
+//   F32 pages: x = h + m + l, three bf16 cut off one after the other (8 bits each: exact
+//   down to 2^-110, below it to bf16's smallest step, 2^-133), and six of the nine products:
+//   hh, hm, mh, mm, hl, lh (the other three are below 2^-21 of |x y|, 2^-24 as a rule);
+//   6/16 of the fp32 matrix rate's time.
 //   F16 pages: K and V are fp16 as they are; q (scaled by a power of two a row) is
 //   h + 2^-12 l, two fp16 parts with a sum of their own each, 22 bits of every element;
 //   p (times 2^15) is h + l with one sum, 22 bits down to p = 2^-16 and 2^-39 below
@@ -65,7 +66,9 @@ __device__ __forceinline__ float q_value(const PagedArgs& a, long row, int h, in
 // Infinities and NaN do not split, and 0 times one of them in a masked place is NaN: a
 // row whose result is not finite is done again in plain fp32 (row_careful, by the
 // joining kernel), where masked places are left out.  So is a row whose scores are too
-// far out (far_out), whose result is made NaN.
+// far out (far_out) or, with F32 pages, whose q has elements that 2^-133 is not small
+// beside (q_splits): their results are made NaN.  And, with F32 pages, one with an element
+// below kSmall, where V's lost digits would show.
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
@@ -205,6 +208,14 @@ struct Parts<_Float16> {
 __device__ __forceinline__ bool far_out(float top) {
     return fabsf(top) > 4194304.f && top != -INFINITY;
 }
+
+// Whether F32 pages' three parts hold a score's digits: q's elements are 0 or from 2^-100 to
+// 2^100, so that its own last steps, and 2^-133 of a key's element times it, are below
+// 2^-33.  high: the largest |element|; low: the least of their bits less one (of 0: all ones).
+__device__ __forceinline__ bool q_splits(float high, uint32_t low) {
+    return high <= 0x1p100f && low >= 0x0d7fffffu;  // 2^-100 is 0x0d800000
+}
+constexpr float kSmall = 0x1p-100f;
 
 // Reductions over the four 16-lane rows of a wave (lanes n, n + 16, n + 32, n + 48),
 // every lane receiving the result.  v_permlane{16,32}_swap of a value with itself
@@ -488,6 +499,18 @@ __device__ __forceinline__ void load_q(const PagedArgs& a, const Span& sp, int r
         const int ex = top > 0.f ? min(max(15 - (int)__builtin_amdgcn_frexp_expf(top), -100), 100) : 0;
         up = __builtin_ldexpf(1.f, ex);
         scale = __builtin_ldexpf(scale, -ex);
+    } else {
+        float high = 0.f;
+        uint32_t low = ~0u;
+#pragma unroll
+        for (int c = 0; c < NC; c++)
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                high = fmaxf(high, fabsf(x[c][e]));
+                low = min(low, (__float_as_uint(x[c][e]) & 0x7fffffffu) - 1u);
+            }
+        // NaN of one lane reaches O and the weights' sum from its keys
+        scale = q_splits(high, low) ? scale : NAN;
     }
 #pragma unroll
     for (int c = 0; c < NC; c++) {
@@ -1123,9 +1146,13 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
         for (int e = 0; e < E; e++) o[e] *= by;
     }
     float check = l * 0.f;
+    bool small = false;
 #pragma unroll
-    for (int e = 0; e < E; e++) check = fmaf(o[e], 0.f, check);
-    const bool again = __any(check != 0.f);
+    for (int e = 0; e < E; e++) {
+        check = fmaf(o[e], 0.f, check);
+        if (sizeof(T) == 4) small |= fabsf(o[e]) < kSmall && o[e] != 0.f;
+    }
+    const bool again = __any(check != 0.f || small);
     if (again) row_careful<HD, T>(a, s, i, h, o);
     if (again || w1 != w2) {
 #pragma unroll

@@ -34,3 +34,38 @@ def test_large_scores(ctx, heads, kvh, hd, tok, kv, std):
         assert np.all(np.abs(got - want)[sure] <= 12 * U * size[sure] + low)
 
 
+@pytest.mark.parametrize("tok", [1, 12, 40])
+@pytest.mark.parametrize("hd", [64, 128, 256])
+def test_small_values(ctx, hd, tok):
+    """Values down to the end of fp32's normal range keep their digits."""
+    c = Case(61, 4, 2, hd, "f32", 16, [90, 33], [tok, tok], tok, rope=False)
+    c.v *= (10.0 ** np.linspace(-36.5, -29, hd)).astype(np.float32)
+    want, size = c.want()
+    live = np.arange(tok)[None] < c.n_tok[:, None]
+    for max_len in (90, 0):
+        a, b = c.run(ctx, max_len=max_len)[live], want[live]
+        # as Case.check: scores of at most 60 off by (hd + 6) U of their terms; below 2^-126
+        # fp32 itself steps by 2^-149, at most once a row summed
+        per = 2 * ((hd + 6) * U * 60 + (90 + tok + 16) * U)
+        assert np.all(np.abs(a - b) <= per * size[live] + 200 * 2.0 ** -149)
+        rel = np.abs(a - b) / size[live]
+        assert np.sqrt(np.mean(rel ** 2)) <= 2e-6
+
+
+@pytest.mark.parametrize("tok", [1, 12, 40])
+@pytest.mark.parametrize("low,high", [(-36, -30), (30, 36)])
+def test_keys_at_the_ends(ctx, low, high, tok):
+    """Keys of 1e-36 or 1e36 next to ordinary ones, under queries that even them out: no
+    score loses a term's digits."""
+    c = Case(67, 4, 2, 128, "f32", 16, [90, 33], [tok, tok], tok, rope=False)
+    scale = np.ones(128, np.float32)
+    scale[::2] = (10.0 ** np.linspace(low, high, 64)).astype(np.float32)
+    c.k *= scale
+    c.q /= scale
+    want, size = c.want()
+    live = np.arange(tok)[None] < c.n_tok[:, None]
+    a, b = c.run(ctx)[live], want[live]
+    # per score: (hd + 6) U sum|q_d k_d| / sqrt(hd), |q_d k_d| at most 6 sigma squares apart
+    assert np.all(np.abs(a - b) <= 2 * (134 * U * 40 + 150 * U) * size[live])
+    rel = np.abs(a - b) / size[live]
+    assert np.sqrt(np.mean(rel ** 2)) <= 2e-6
