@@ -347,8 +347,9 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
 /* Beam search's selection: of all continuations of n_beams beams a sequence the
  * n_out best.  Beam b of sequence s has logits row s * n_beams + b (ld floats
  * apart) and the score cum[s * n_beams + b]; its continuation by token t scores
- * cum + (x[t] - log sum exp x), in 64 bits.  They rank by score, then lower
- * beam, higher logit, lower token.  done (may be NULL): a beam with done != 0 has
+ * cum + (x[t] - log sum exp x), in 64 bits (each exponential within 3e-15 of itself;
+ * cum is the fp32 that it is, and score is rounded to fp32 once the ranks are known).
+ * They rank by score, then lower beam, higher logit, lower token.  done (may be NULL): a beam with done != 0 has
  * one continuation, eos_id, that keeps its score.  A score of -inf or NaN (a
  * masked token, an unused beam with cum -inf; a row with a NaN or +inf logit) is
  * no continuation.  token, parent (the beam, 0..n_beams-1) and score: n_out a

@@ -185,3 +185,31 @@ def test_same_bits_each_time(ctx):
     for _ in range(3):
         b = run(ctx, x, cum, None, -1, 16)
         assert all(np.array_equal(p.view(np.uint32), q.view(np.uint32)) for p, q in zip(a, b))
+
+
+def test_closest_scores(ctx):
+    """Pairs of beams some 1e-13 apart, by exponentials of unlike arguments: log(1 + e^a) against
+    log(1 + e^b + e^c + e^d)."""
+    rng = np.random.default_rng(9)
+    n = 1024
+    e64 = lambda v: np.exp(v.astype(np.float64))  # noqa: E731
+    a = -0.01 - 0.7 * rng.random(n).astype(np.float32)
+    b = a + np.log(0.2 + 0.6 * rng.random(n)).astype(np.float32)
+    c = np.log(e64(a) - e64(b) - 4e-7).astype(np.float32)
+    # what is left of e^a: d's fp32 steps, 9.5e-7, are some 4e-13 of the sum
+    d = np.log(e64(a) - e64(b) - e64(c)).astype(np.float32)
+    x = np.full((n, 2, 4), -np.inf, np.float32)
+    x[:, 0, 0], x[:, 0, 1] = 0, a
+    x[:, 1] = np.stack([np.zeros(n, np.float32), b, c, d], 1)
+    lse = np.log(np.exp(x.astype(np.float64)).sum(-1))
+    gap = np.abs(lse[:, 0] - lse[:, 1])
+    # exponentials to 3e-15 of their values, sums and logarithms of at most 1.1 to 1e-15 more
+    pick = np.flatnonzero((gap > 2e-14) & (gap < 5e-13))
+    assert len(pick) > n // 2, len(pick)
+    x = np.ascontiguousarray(x[pick])
+    cum = np.zeros((len(pick), 2), np.float32)
+    got = run(ctx, x, cum, None, -1, 2)
+    first = (lse[pick, 1] < lse[pick, 0]).astype(np.int32)
+    assert not got[0].any()
+    assert np.array_equal(got[1], np.stack([first, 1 - first], 1)), (
+        np.count_nonzero(got[1][:, 0] != first), len(pick))
