@@ -291,7 +291,7 @@ int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n)
  *     is -1.  What the input tables held and no output holds is free again.
  *   - parent[i] outside 0..n_in-1 or len[i] < 0: sequence i holds nothing.
  * A text starts as an input row of -1 with len 0.  table_out: n_out rows of
- * table_ld entries, entries past the room -1, not the array `table`.  refs_out
+ * table_ld entries (below 2^31 in all), entries past the room -1, not the array `table`.  refs_out
  * (n_pages) may be refs; refs has to count what the tables hold.  info (3 int32):
  * copied pages, entries left without a page, pages free afterwards.  Room past
  * table_ld pages is cut off there. */
