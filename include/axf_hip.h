@@ -294,7 +294,7 @@ int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n)
  * table_ld entries (below 2^31 in all), entries past the room -1, not the array `table`.  refs_out
  * (n_pages) may be refs; refs has to count what the tables hold.  info (3 int32):
  * copied pages, entries left without a page, pages free afterwards.  Room past
- * table_ld pages is cut off there. */
+ * table_ld pages is cut off there.  n_pages up to 2^30. */
 int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, int32_t* refs_out,
                     int32_t* info, const int32_t* table, const int32_t* refs, int n_in,
                     const int32_t* parent, const int32_t* len, int n_out, int table_ld, int extra);

@@ -69,6 +69,8 @@ int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, in
     AXF_REQUIRE(n_in >= 0 && n_out >= 0 && n_in <= 65536 && n_out <= 65536,
                 "up to 65536 sequences");
     AXF_REQUIRE(table_ok(kv, table_ld), "bad table_ld");
+    // the kernel steps over its pages, 4096 at a time, in 32 bits
+    AXF_REQUIRE(kv->n_pages <= (1 << 30), "a pool of more than 2^30 pages");
     // the kernel counts pages to take in 32 bits
     AXF_REQUIRE((long)n_out * table_ld < (1L << 31), "table_out of 2^31 entries or more");
     AXF_REQUIRE(extra >= 0 && extra <= (1 << 30), "bad extra");

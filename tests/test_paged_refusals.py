@@ -65,3 +65,11 @@ def test_fork_counts_its_entries_in_32_bits(n_out, table_ld):
 def test_fork_just_below():
     rc, said = call("axf_hip_kv_fork", n_out=65536, table_ld=(1 << 15) - 1, extra=1 << 19)
     assert rc == _ffi.AXF_ERR_HIP, (rc, said)
+
+
+def test_fork_walks_its_pool_in_32_bits():
+    big = dict(kv_page_rows=1, kv_n_kv_heads=1, kv_head_dim=64, kv_type=1, kv_n_layers=1)
+    refused("axf_hip_kv_fork", "2^30 pages", kv_n_pages=(1 << 30) + 1, **big)
+    refused("axf_hip_kv_fork", "2^30 pages", kv_n_pages=(1 << 31) - 1, **big)
+    rc, said = call("axf_hip_kv_fork", kv_n_pages=1 << 20, **big)
+    assert rc == _ffi.AXF_ERR_HIP, (rc, said)
