@@ -265,7 +265,9 @@ int axf_hip_embed(axf_ctx* ctx, float* out, int qtype, const void* W, int token,
  * convention) holds no rows: reads see nothing there and writes are dropped.
  * type: AXF_TYPE_F32 or AXF_TYPE_F16; page_rows: a power of two up to 1024;
  * head_dim 64, 128 or 256; k and v 16-byte aligned.  Integer arrays (table, len,
- * n_tok, pos, ...) are device memory, so that a step needs no host round trip. */
+ * n_tok, pos, ...) are device memory.  What a call writes (of k and v: the layer's rows,
+ * or all of them in fork and compaction) overlaps nothing else that it reads or writes,
+ * but for refs_out = refs, len_out = len and, with n_out = n_beams, score = cum. */
 typedef struct {
     void* k;
     void* v;

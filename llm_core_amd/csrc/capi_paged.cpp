@@ -2,6 +2,7 @@
 // (declared in include/axf_hip.h; kernels in kernels/paged.hip, kernels/beam.hip).
 #include "capi_check.hpp"
 
+#include <initializer_list>
 #include <string>
 
 using namespace axf;
@@ -31,11 +32,33 @@ size_t layer_bytes(const axf_kv_pages* kv) {
            (kv->type == AXF_TYPE_F32 ? 4 : 2);
 }
 
-// Whether two arrays have memory in common.
-bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
-    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
-    return x < y + b_bytes && y < x + a_bytes;
+// An argument's array, for fault messages by name.  None (a null pointer) has no bytes.
+struct Array {
+    const char* name;
+    const void* p;
+    size_t bytes;
+};
+
+// What is wrong where a call writes arrays that it also reads (other workgroups may do so
+// later) or writes as something else: empty if nothing.
+std::string overlap_fault(std::initializer_list<Array> writes, std::initializer_list<Array> reads) {
+    auto common = [](const Array& a, const Array& b) {
+        const uintptr_t x = reinterpret_cast<uintptr_t>(a.p), y = reinterpret_cast<uintptr_t>(b.p);
+        return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+    };
+    for (const Array* w = writes.begin(); w != writes.end(); w++) {
+        for (const Array* o = w + 1; o != writes.end(); o++)
+            if (common(*w, *o)) return std::string(w->name) + " must not overlap " + o->name;
+        for (const Array& r : reads)
+            if (common(*w, r)) return std::string(w->name) + " must not overlap " + r.name;
+    }
+    return {};
 }
+#define AXF_REQUIRE_APART(...)                                            \
+    do {                                                                  \
+        const std::string fault_ = overlap_fault(__VA_ARGS__);            \
+        AXF_REQUIRE(fault_.empty(), fault_);                              \
+    } while (0)
 
 // Positions are 32-bit.
 bool table_ok(const axf_kv_pages* kv, int table_ld) {
@@ -77,15 +100,21 @@ int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, in
     AXF_REQUIRE(refs && refs_out && info && (n_in == 0 || table) &&
                     (n_out == 0 || (table_out && parent && len)),
                 "null pointer");
-    AXF_REQUIRE(!overlap(table_out, (size_t)n_out * table_ld * 4, table, (size_t)n_in * table_ld * 4),
-                "table_out must not overlap table");
-    AXF_REQUIRE(refs_out == refs ||
-                    !overlap(refs_out, (size_t)kv->n_pages * 4, refs, (size_t)kv->n_pages * 4),
-                "refs_out must be refs or apart from it");
     AXF_REQUIRE(aligned(table, 4) && aligned(table_out, 4) && aligned(refs, 4) &&
                     aligned(refs_out, 4) && aligned(info, 4) && aligned(parent, 4) &&
                     aligned(len, 4),
                 "misaligned pointer");
+    const size_t entry = (size_t)table_ld * 4, seqs = (size_t)n_out * 4;
+    const size_t pool = extra > 0 ? kv->n_layers * layer_bytes(kv) : 0;  // 0: not touched
+    AXF_REQUIRE_APART({{"table_out", table_out, n_out * entry},
+                       {"refs_out", refs_out, (size_t)kv->n_pages * 4},
+                       {"info", info, 12},
+                       {"k", pool ? kv->k : nullptr, pool},
+                       {"v", pool ? kv->v : nullptr, pool}},
+                      {{"table", table, n_in * entry},
+                       {"refs", refs == refs_out ? nullptr : refs, (size_t)kv->n_pages * 4},
+                       {"parent", parent, seqs},
+                       {"len", len, seqs}});
     DeviceScope device(ctx);
     void* scratch = nullptr;
     int rc = ctx_scratch(ctx, kv_fork_scratch(kv->n_pages, n_out), &scratch);
@@ -129,10 +158,25 @@ int axf_hip_kv_store(axf_ctx* ctx, const axf_kv_pages* kv, int layer, const int3
                     aligned(v, 4) && aligned(bk, 4) && aligned(bv, 4) && aligned(pos, 4) &&
                     aligned(cos_t, 4) && aligned(sin_t, 4),
                 "misaligned pointer");
+    const size_t bytes = layer_bytes(kv), rows = (size_t)n_seq * max_tok, seqs = (size_t)n_seq * 4;
+    const size_t turns = (size_t)n_pos * (kv->head_dim / 2) * 4;
+    char* const k_at = static_cast<char*>(kv->k) + layer * bytes;
+    char* const v_at = static_cast<char*>(kv->v) + layer * bytes;
+    AXF_REQUIRE_APART({{"the pages' k", k_at, bytes}, {"the pages' v", v_at, bytes}},
+                      {{"table", table, seqs * table_ld},
+                       {"len", len, seqs},
+                       {"n_tok", n_tok, seqs},
+                       {"k", k, ((rows - 1) * k_ld + row) * 4},
+                       {"bk", bk, (size_t)row * 4},
+                       {"v", v, ((rows - 1) * v_ld + row) * 4},
+                       {"bv", bv, (size_t)row * 4},
+                       {"pos", pos, rows * 4},
+                       {"cos_t", pos ? cos_t : nullptr, turns},
+                       {"sin_t", pos ? sin_t : nullptr, turns}});
     DeviceScope device(ctx);
     KvStoreArgs a{};
-    a.k = static_cast<char*>(kv->k) + layer * layer_bytes(kv);
-    a.v = static_cast<char*>(kv->v) + layer * layer_bytes(kv);
+    a.k = k_at;
+    a.v = v_at;
     a.table = table;
     a.table_ld = table_ld;
     a.len = len;
@@ -175,21 +219,34 @@ int axf_hip_attn_paged(axf_ctx* ctx, float* out, void* outq8, const float* q, in
     AXF_REQUIRE(out && q && table && len, "null pointer");
     AXF_REQUIRE(!pos || (cos_t && sin_t && n_pos > 0), "pos needs the RoPE tables");
     AXF_REQUIRE(q_ld >= n_heads * kv->head_dim, "q_ld below one row");
-    const size_t rows = (size_t)n_seq * max_tok;
-    AXF_REQUIRE(!overlap(out, rows * n_heads * kv->head_dim * 4, q,
-                         ((rows - 1) * q_ld + (size_t)n_heads * kv->head_dim) * 4),
-                "out must not overlap q");
     AXF_REQUIRE(aligned(out, 4) && aligned(outq8, 4) && aligned(q, 4) && aligned(bq, 4) &&
                     aligned(table, 4) && aligned(len, 4) && aligned(n_tok, 4) &&
                     aligned(mask, 8) && aligned(pos, 4) && aligned(cos_t, 4) && aligned(sin_t, 4),
                 "misaligned pointer");
+    const size_t rows = (size_t)n_seq * max_tok, row = (size_t)n_heads * kv->head_dim;
+    const size_t bytes = layer_bytes(kv), seqs = (size_t)n_seq * 4;
+    const size_t turns = (size_t)n_pos * (kv->head_dim / 2) * 4;
+    const char* const k_at = static_cast<const char*>(kv->k) + layer * bytes;
+    const char* const v_at = static_cast<const char*>(kv->v) + layer * bytes;
+    AXF_REQUIRE_APART({{"out", out, rows * row * 4}, {"outq8", outq8, rows * (row / 32) * Q8_0_BYTES}},
+                      {{"q", q, ((rows - 1) * q_ld + row) * 4},
+                       {"bq", bq, row * 4},
+                       {"the pages' k", k_at, bytes},
+                       {"the pages' v", v_at, bytes},
+                       {"table", table, seqs * table_ld},
+                       {"len", len, seqs},
+                       {"n_tok", n_tok, seqs},
+                       {"mask", mask, rows * 8},
+                       {"pos", pos, rows * 4},
+                       {"cos_t", pos ? cos_t : nullptr, turns},
+                       {"sin_t", pos ? sin_t : nullptr, turns}});
     DeviceScope device(ctx);
     PagedArgs a{};
     a.q = q;
     a.q_ld = q_ld;
     a.bq = bq;
-    a.k = static_cast<const char*>(kv->k) + layer * layer_bytes(kv);
-    a.v = static_cast<const char*>(kv->v) + layer * layer_bytes(kv);
+    a.k = k_at;
+    a.v = v_at;
     a.table = table;
     a.table_ld = table_ld;
     a.len = len;
@@ -226,11 +283,18 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
     AXF_REQUIRE(n_seq >= 0 && n_seq <= 65535, "bad n_seq");
     if (n_seq == 0) return AXF_OK;
     AXF_REQUIRE(len_out && table && len && n_path && (path || max_path == 0), "null pointer");
-    AXF_REQUIRE(len_out == len || !overlap(len_out, (size_t)n_seq * 4, len, (size_t)n_seq * 4),
-                "len_out must be len or apart from it");
     AXF_REQUIRE(aligned(len_out, 4) && aligned(table, 4) && aligned(len, 4) && aligned(path, 4) &&
                     aligned(n_path, 4),
                 "misaligned pointer");
+    const size_t seqs = (size_t)n_seq * 4;
+    const size_t pool = max_path > 0 ? kv->n_layers * layer_bytes(kv) : 0;  // 0: not touched
+    AXF_REQUIRE_APART({{"len_out", len_out, seqs},
+                       {"k", pool ? kv->k : nullptr, pool},
+                       {"v", pool ? kv->v : nullptr, pool}},
+                      {{"table", table, seqs * table_ld},
+                       {"len", len == len_out ? nullptr : len, seqs},
+                       {"path", path, seqs * max_path},
+                       {"n_path", n_path, seqs}});
     DeviceScope device(ctx);
     AXF_HIP(launch_kv_compact(*kv, len_out, table, table_ld, len, path, n_path, n_seq, max_path,
                               ctx->stream));
@@ -248,13 +312,15 @@ int axf_hip_beam_select(axf_ctx* ctx, int32_t* token, int32_t* parent, float* sc
     AXF_REQUIRE(ld >= n_vocab, "ld below one row");
     if (n_seq == 0) return AXF_OK;
     AXF_REQUIRE(token && parent && score && logits && cum, "null pointer");
-    AXF_REQUIRE((score == cum && n_out == n_beams) ||
-                    !overlap(score, (size_t)n_seq * n_out * 4, cum, (size_t)n_seq * n_beams * 4),
-                "score must be cum (with n_out = n_beams) or apart from it");
     AXF_REQUIRE(!done || (eos_id >= 0 && eos_id < n_vocab), "eos_id out of range");
     AXF_REQUIRE(aligned(token, 4) && aligned(parent, 4) && aligned(score, 4) &&
                     aligned(logits, 4) && aligned(cum, 4) && aligned(done, 4),
                 "misaligned pointer");
+    const size_t rows = (size_t)n_seq * n_beams, kept = (size_t)n_seq * n_out * 4;
+    AXF_REQUIRE_APART({{"token", token, kept}, {"parent", parent, kept}, {"score", score, kept}},
+                      {{"logits", logits, ((rows - 1) * ld + n_vocab) * 4},
+                       {"cum", score == cum && n_out == n_beams ? nullptr : cum, rows * 4},
+                       {"done", done, rows * 4}});
     DeviceScope device(ctx);
     BeamArgs a{};
     a.token = token;
