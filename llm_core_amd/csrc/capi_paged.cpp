@@ -71,13 +71,16 @@ extern "C" {
 
 int axf_tree_masks(uint64_t* mask, int32_t* depth, const int32_t* parent, int n) {
     AXF_REQUIRE(mask && parent && n > 0 && n <= 64, "bad arguments (1 to 64 nodes)");
-    for (int i = 0; i < n; i++)
-        AXF_REQUIRE(parent[i] >= -1 && parent[i] < i, "a node's parent must come before it");
+    uint64_t m[64];  // written once parent is read: it may be the same memory
     int32_t d[64];
     for (int i = 0; i < n; i++) {
         const int32_t p = parent[i];
-        mask[i] = (1ull << i) | (p >= 0 ? mask[p] : 0);
+        AXF_REQUIRE(p >= -1 && p < i, "a node's parent must come before it");
+        m[i] = (1ull << i) | (p >= 0 ? m[p] : 0);
         d[i] = p >= 0 ? d[p] + 1 : 0;
+    }
+    for (int i = 0; i < n; i++) {
+        mask[i] = m[i];
         if (depth) depth[i] = d[i];
     }
     return AXF_OK;

@@ -159,3 +159,18 @@ def test_fork_walks_its_pool_in_32_bits():
     refused("axf_hip_kv_fork", "2^30 pages", kv_n_pages=(1 << 31) - 1, **big)
     rc, said = call("axf_hip_kv_fork", kv_n_pages=1 << 20, **big)
     assert rc == _ffi.AXF_ERR_HIP, (rc, said)
+
+
+def test_tree_masks_over_the_parents():
+    """One array for a tree's parents and what is made of them."""
+    both = (C.c_uint64 * 64)()
+    parent = C.cast(both, C.POINTER(C.c_int32))
+    for i, p in enumerate([-1, -1, 1, -1]):
+        parent[i] = p
+    depth = (C.c_int32 * 4)()
+    assert _ffi.lib.axf_tree_masks(both, depth, both, 4) == 0
+    assert list(both[:4]) == [1, 2, 6, 8] and list(depth) == [0, 0, 1, 0]
+    tree = (C.c_int32 * 4)(-1, 0, 1, 0)
+    mask = (C.c_uint64 * 4)()
+    assert _ffi.lib.axf_tree_masks(mask, tree, tree, 4) == 0
+    assert list(mask) == [1, 3, 7, 9] and list(tree) == [0, 1, 2, 1]
