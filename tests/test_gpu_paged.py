@@ -169,6 +169,26 @@ def test_attn_q8(ctx, tok):
 
 
 @pytest.mark.parametrize("kv", ["f32", "f16"])
+@pytest.mark.parametrize("heads,kvh,hd", [(6, 3, 64), (8, 2, 128), (4, 2, 256)])
+@pytest.mark.parametrize("tok", [1, 5, 40])
+def test_attn_q8_of_all_heads(ctx, heads, kvh, hd, tok, kv):
+    """Q8_0 blocks of every head dimension and page type; a row that sees nothing is blocks of
+    zeros."""
+    c = Case(hd + tok, heads, kvh, hd, kv, 16, [300, 0, 0], [tok, 1, max(1, tok // 2)], tok)
+    c.mask[1, 0] = 0
+    for max_len in (300, 0):
+        got, q8 = c.run(ctx, q8=True, max_len=max_len)
+        c.check(got, *c.want())
+        assert not got[1, 0].any() and not q8[1, 0].any()
+        for s in range(c.n):
+            for i in range(c.max_tok):
+                if i < c.n_tok[s]:
+                    assert np.array_equal(q8[s, i], O.quantize_q8_0(got[s, i].reshape(-1)))
+                else:
+                    assert np.all(q8[s, i] == 0xa5)
+
+
+@pytest.mark.parametrize("kv", ["f32", "f16"])
 @pytest.mark.parametrize("tok", [1, 7, 40])
 def test_attn_masked_places_change_nothing(ctx, tok, kv):
     """NaN and infinities in unused rows of used pages, in unused pages, in other layers and in
