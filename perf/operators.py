@@ -24,7 +24,9 @@ _ctx = None
 
 
 def _context():
-    """The program's one device context (one in-order stream)."""
+    """The program's one device context.  Its in-order stream is its own, not torch's: what
+    torch still computes is waited for before the first call (prepare), and what the calls
+    compute (Context.sync, or torch.cuda.synchronize) before torch reads or frees it."""
     global _ctx
     if _ctx is None:
         from llm_core_amd import hip
@@ -212,6 +214,13 @@ def _rope(s, head_dim, n_pos):
 
 
 def prepare(case, seed):
+    s = _inputs(case, seed)
+    if own:
+        torch.cuda.synchronize()  # the library's calls run on a stream of their own
+    return s
+
+
+def _inputs(case, seed):
     r = random.Random(int(seed) * 6007 + 5)
     g = torch.Generator(device=DEV)
     g.manual_seed(int(seed) * 7919 + 17)
