@@ -13,6 +13,9 @@
  *     enqueue asynchronously on that stream; axf_hip_sync and the d2h copy
  *     block.  Pointer arguments named W, x, y, xq8, ... are device pointers
  *     owned by the caller (allocated with axf_hip_alloc or any HIP allocator).
+ *     The stream is the context's own and is ordered with no other: what other
+ *     streams still do to a call's arrays has to be waited for before the call,
+ *     and the call before they read, write or free them.
  *   - Weights are GGUF super-blocks in their native layout: Q4_K 144 B and
  *     Q6_K 210 B per 256 weights (reference include/axonforge/dtype.hpp:136-155),
  *     rows contiguous, row r at W + r*row_bytes.
@@ -267,7 +270,9 @@ int axf_hip_embed(axf_ctx* ctx, float* out, int qtype, const void* W, int token,
  * head_dim 64, 128 or 256; k and v 16-byte aligned.  Integer arrays (table, len,
  * n_tok, pos, ...) are device memory.  What a call writes (of k and v: the layer's rows,
  * or all of them in fork and compaction) overlaps nothing else that it reads or writes,
- * but for refs_out = refs, len_out = len and, with n_out = n_beams, score = cum. */
+ * but for refs_out = refs, len_out = len and, with n_out = n_beams, score = cum.  fork,
+ * attention and selection keep a workspace of the context, allocated when a call first
+ * needs as much. */
 typedef struct {
     void* k;
     void* v;
@@ -349,8 +354,8 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
 /* Beam search's selection: of all continuations of n_beams beams a sequence the
  * n_out best.  Beam b of sequence s has logits row s * n_beams + b (ld floats
  * apart) and the score cum[s * n_beams + b]; its continuation by token t scores
- * cum + (x[t] - log sum exp x), in 64 bits (each exponential within 3e-15 of itself;
- * cum is the fp32 that it is, and score is rounded to fp32 once the ranks are known).
+ * cum + (x[t] - log sum exp x), in 64 bits (exp(-d) within 3e-15 + d 2^-54 of itself; cum
+ * is the fp32 that it is, and score is rounded to fp32 once the ranks are known).
  * They rank by score, then lower beam, higher logit, lower token.  done (may be NULL): a beam with done != 0 has
  * one continuation, eos_id, that keeps its score.  A score of -inf or NaN (a
  * masked token, an unused beam with cum -inf; a row with a NaN or +inf logit) is

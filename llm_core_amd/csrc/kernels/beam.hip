@@ -4,17 +4,19 @@
 //   score(b, t) = cum[b] + (x[b][t] - lse[b]),  lse[b] = log sum_t exp x[b][t]
 //
 // Which of two continuations is better may hang on the last bits of a score, so
-// exponentials, sums and scores are 64-bit (the fp64 units run at the fp32 rate
-// here, and a logit costs some 20 operations against 4 bytes from HBM).  Within a
-// beam the score rises with the logit, so one pass over the logits suffices:
+// exponentials, sums and scores are 64-bit.  Within a beam the score rises with the
+// logit, so one pass over the logits suffices:
 //   1. k_beam_part: a workgroup takes a chunk of a row: its maximum m, sum of
 //      exp(x - m) and its n_out largest (logit, lower token first) keys.
 //   2. k_beam_merge: a workgroup a sequence joins the chunks' sums to each beam's
 //      lse, turns the keys into scores and picks the n_out best of the chunks' sorted
 //      lists.
-// 8 x 8 beams of 151936 (38.9 MB, 7.5 us at a large copy's rate): 17.6 + 10.2 us; the
-// first is bound by the 64-bit arithmetic (9.7 million logits at about 20 operations), the
-// second by the latencies of one workgroup a sequence.  1 x 4 of 32000: 4.1 + 5.6 us.
+// 8 x 8 beams of 151936 (38.9 MB, 7.5 us at a large copy's rate): 18.4 + 11.2 us (medians
+// of a kernel trace).  The first: 38 vector instructions a logit, the 64-bit ones among
+// them at half rate; the vector units are busy 63% of its time, the rest is ramp, loads and
+// the 32 dependent ballots ahead of them (waves wait 44%).  The second: the latencies of one
+// workgroup a sequence.  1 x 4 of 32000: 5.0 + 6.3 us.  A finished beam's row is read and
+// summed like the others.
 #include "common.hpp"
 
 namespace axf {

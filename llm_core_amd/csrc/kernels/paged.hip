@@ -304,8 +304,10 @@ __device__ __forceinline__ long div_whole(long a, long b) {
 
 // A unit is `per` steps of 32 keys.  With per 3 a last tile at most half full has units of
 // 4 steps: its waves without rows leave the others the SIMDs, and a step takes 0.74 of a
-// full tile's time (16 sequences @8000, 64 and 128 rows: 275 and 368 us).  48 tokens (192
-// rows): 593 us, with units of 3 steps for both 618, of 1 618.
+// full tile's time (16 sequences @8000, 64 and 128 rows: 275 and 368 us).  48 tokens of 16
+// sequences @8000 (192 rows), with 4 and with 3 steps: 128 elements a head F32 592 and 610 us,
+// F16 327 and 356; 64 elements F32 375 and 412; 256 elements F16 259 and 266, F32 904 and
+// 892 (@2000: 253 and 260).
 struct SeqWork {
     int rows, tiles, per_last;
     long units, last;  // of a part, of one of the last row tile
@@ -594,12 +596,13 @@ __device__ __forceinline__ void for_spans(const PagedArgs& a, int tile_rows, Bod
 // V: 8 keys of HD/16 consecutive elements), no LDS in between.  The workgroup's four
 // waves take every fourth step of the split and join at its end.
 //
-// Bound by HBM where the cache is long: 16 sequences @4000 of 32/8 heads of 128, one token:
-// F32 71.6 us (4.6 TB/s), F16 43.0 (3.8 TB/s; half the bytes for the same steps).  One
-// token @1024 (24 workgroups) is a chain of latencies, 11.5 us + 3.9 of the join: 1.6 to
-// start, 1 for the lengths' plan, 1.2 for the span, 2.6 and 1.9 for the table's and then
-// K's and q's loads, 3.1 for the step's arithmetic (splits, products and softmax of one
-// wave a SIMD), 1.1 to join the waves.
+// Bound by HBM where the cache is long: 16 sequences of 4000 rows, 32/8 heads of 128, one
+// token: F32 (525 MB) 96.6 us, 5.4 TB/s; F16 56.5 us, 4.6 TB/s (half the bytes for the same
+// steps); 256 elements, 16/4 heads, F32 120 us, 4.4 TB/s (48 registers spilt, 188 bytes a
+// lane).  One token @1024 (24 workgroups) is a chain of latencies, 11.9 us + 4.3 of the
+// join: 1.6 to start, 1 for the lengths' plan, 1.2 for the span, 2.6 and 1.9 for the table's
+// and then K's and q's loads, 3.1 for the step's arithmetic (splits, products and softmax of
+// one wave a SIMD), 1.1 to join the waves.
 constexpr int kFewWaves = 4;
 
 template <int HD, class T>
@@ -797,12 +800,17 @@ __global__ __launch_bounds__(64 * kFewWaves) void k_attn_paged_few(PagedArgs a) 
 // 64 rows of 4 waves, two workgroups a CU, else 128 or 256 of 8 waves.  The next step's
 // values are in flight while this one is multiplied.
 //
-// 16 trees of up to 48 tokens, 32/8 heads of 128 @8191, F32: 380 us, 129 TFLOP/s of scores
-// and sums where six bf16 products a value allow 200 at a large library product's rate
-// (243 us).  What bounds it is no one unit; of 402 us before its last steps, with half the
-// products 307, without the splitting 371, with a third of the LDS reads 375, without
-// loads 360, loads and splitting alone 231.  The two waves of a SIMD go through the step's phases together,
-// between the same barriers.  Tried: K of the next step multiplied under this one's
+// 16 trees of up to 48 tokens, 32/8 heads of 128 @8191, F32: 360 to 375 us called in a row,
+// 375 to 488 (median 446, at some 1.7 GHz) launched one by one under the profiler; 243 us is
+// what six bf16 products a value take at a large library product's rate.  No one unit bounds
+// it: vector units busy 45%, matrix units 37%, waves waiting 31% of the time.  Of 402 us
+// before its last steps, with half the products 307, without the splitting 371, with a third
+// of the LDS reads 375, without loads 360, loads and splitting alone 231.  The two waves of
+// a SIMD go through the step's phases together, between the same barriers.  F16 pages, 28/4
+// heads, 48 tokens @8000: 128 elements 306 us (vector units 50%, matrix units 24%, waiting
+// 36%), 64 elements 275 us (41%, 12%, 46%; 11.6 vector instructions a product: softmax and
+// the splitting of p).  256 elements, F32, 16/4 heads, 48 tokens @4000: 464 us (24%, 23%,
+// 62%; 50 registers spilt, 188 bytes a lane).  Tried: K of the next step multiplied under this one's
 // softmax (427), one LDS buffer and 2 workgroups (419), raised priority around the
 // products (400), 4 waves of three tiles (158 registers spilt, 822).
 
@@ -1073,9 +1081,10 @@ void k_attn_paged_many(PagedArgs a) {
 // One wave a query row and head.  Where its part lies in several shares, their sums are
 // brought to one base and added in their order, and divided by the weights' sum (lane j
 // has share j's m and l, so one load's latency covers 64 of them); a whole part's row
-// is read back.  A row that is not finite is done again with care.  3.9 us for 16 rows, 4.1
-// for 672 (launch and three loads after each other: plan, m and l, sums); 16.3 us for
-// 24576 rows of 128 whose 256 shares' sums are 34 MB.
+// is read back.  A row that is not finite is done again with care, and so is one of F32
+// pages with an element so small that the three parts have lost its digits.  4.3 us for 16
+// rows, 4.4 for 672 (launch and three loads after each other: plan, m and l, sums), 0.4 more
+// with Q8_0 blocks for 512; 19.6 us for 24576 rows of 128 whose 256 shares' sums are 34 MB.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_rows) {
     constexpr int E = HD / 64, U = 8;
@@ -1179,7 +1188,7 @@ __global__ __launch_bounds__(256) void k_attn_paged_join(PagedArgs a, int tile_r
 // ---- store -----------------------------------------------------------------
 // One thread 4 + 4 values of K (a RoPE pair's halves) and of V: element d..d+3 and
 // d+HD/2.. of one head.  Each value is read and written once: 24 sequences of 48 tokens,
-// 8 heads of 128, F16 (14.1 MB) 4.3 us, 3.3 TB/s; 8 rows of 2 heads of 128 3.0 us, a
+// 8 heads of 128, F16 (14.1 MB) 4.1 us, 3.4 TB/s; 8 rows of 2 heads of 128 3.1 us, a
 // launch's time.
 template <int HD, class T>
 __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
@@ -1234,8 +1243,9 @@ __global__ __launch_bounds__(256) void k_kv_store(KvStoreArgs a) {
 // barriers between its steps and no other launch.  Reference counts are atomics (whole
 // numbers, so their order does not matter), in LDS up to kForkLdsPages pages: one CU's
 // scattered atomics to L2 go one a cycle or less, 128 sequences of 49 pages took 19 us
-// with them.  Everything else goes by index order.  4 beams @1000 5.5 us, 16 x 8 @1500
-// 8.7: the walk's steps after each other, each a load's or a scan's latency.
+// with them.  Everything else goes by index order.  4 beams @1000 5.6 us, 16 x 8 @1500
+// 8.7: the walk's steps after each other, each a load's or a scan's latency.  Past what LDS
+// holds it is the atomics: 64 x 2 sequences @12000 in 48448 pages, 192000 entries, 326 us.
 constexpr int kForkThreads = 1024;
 constexpr int kForkLdsPages = 32768;  // 128 KiB
 
@@ -1450,8 +1460,8 @@ __global__ __launch_bounds__(kForkThreads) void k_kv_fork(KvForkArgs a) {
 }
 
 // The copied pages' rows: workgroup (output, layer and K or V, 16 KiB of the page).
-// 128 pages' rows in 24 layers, 12.6 MB read and written again: 5.1 to 6.6 us, 3.8 to 4.9
-// TB/s; 1.8 to 2.4 us where little is copied.
+// 128 pages' rows in 24 layers, 12.6 MB read and written again: 6.0 to 7.6 us, 3.3 to 4.2
+// TB/s; 2.6 us where little is copied.
 constexpr int kCopyBytes = 16384;
 
 __global__ __launch_bounds__(256) void k_kv_copy(uint8_t* k, uint8_t* v, const int* copy,
@@ -1482,8 +1492,9 @@ __device__ __forceinline__ int path_length(const int* way, int most) {
 // Workgroup (sequence, layer, K or V): each thread owns 16-byte columns and moves rows in
 // path order, eight reads at a time.  path[i] >= i and ascending: a row is written
 // only after every read of it (an earlier write goes to a lower row than every later read).
-// 16 trees of 32 nodes in 32 layers of 4 KiB rows, 80 MB: 15.8 to 18 us, 4.4 to 5.1 TB/s,
-// what a large copy reaches; one tree of 16 in 2 layers 2.4 to 3 us, a launch's time.
+// 16 trees of 32 nodes in 32 layers of 4 KiB rows, 80 MB: 16 to 18.7 us (median 17.4, 4.6
+// TB/s), near what a large copy reaches (5.2); one tree of 16 in 2 layers 2.9 us, a launch's
+// time.
 __global__ __launch_bounds__(256) void k_kv_compact(uint8_t* k, uint8_t* v, int* len_out,
                                                     const int* table, int table_ld,
                                                     const int* len, const int* path,
@@ -1534,13 +1545,14 @@ __global__ __launch_bounds__(256) void k_kv_compact_len(int* len_out, const int*
 }
 
 // Query rows of a KV head that a workgroup takes: the fewest that hold them all, up to
-// 128.  Measured against the next larger tile: 16 sequences @4000 of 32/8 heads of 128, F32,
-// one token (4 rows): 71.6 us, 64-row tiles 78.8; 12 tokens (48 rows): 93.3 us, 128-row
-// tiles 103.6.  256 rows (two tiles a wave, each fragment read from LDS once for both; the
+// 128.  Measured against the next larger tile: 16 sequences of 1000 to 4000 rows, 32/8 heads
+// of 128, F32, one token (4 rows): 71.6 us, 64-row tiles 78.8; 12 tokens (48 rows): 93.3 us,
+// 128-row tiles 103.6.  256 rows (two tiles a wave, each fragment read from LDS once for both; the
 // cache read once for them, which L2 gives to 128-row tiles too) pay where the products are
 // the least of a step, 64 elements a head with F16 pages: 16 trees of 48 tokens, 28/4
-// heads @8000: 169.7 us, 128-row tiles 184.1; F16 at 128 elements 191.7 and 190.0, F32 at
-// 64 208.7 and 210.2; F32 at 128, 16 trees @8191 (40 registers spilt) 446 and 402.
+// heads, 2000 to 8000 rows: 169.7 us, 128-row tiles 184.1; F16 at 128 elements 191.7 and
+// 190.0, F32 at 64 208.7 and 210.2; F32 at 128, 16 trees @8191 (40 registers spilt) 446 and
+// 402.
 int tile_rows(int rows, int head_dim, int kv_type) {
     if (rows <= 16) return 16;
     if (rows <= 64) return 64;
@@ -1589,9 +1601,10 @@ hipError_t store_launch(const KvStoreArgs& a, hipStream_t st) {
 // Workgroups of the launch: as many as run at once, or as few as have a unit each by the
 // caller's estimate of the lengths.  A CU holds two workgroups of 64-row tiles (with F32 at
 // 256 elements one: LDS), or of few rows at 64 elements a head (fewer than 256 registers);
-// one of few rows at 128 and 256 elements, or of 8 waves.  More than run at once leave the last ones a CU to
-// themselves: 16 sequences of 32/8 heads @4000 with 256, 512, 1024 workgroups: 73, 83,
-// 98 us; 12 tokens each, 16/4 heads of 256, F32 (96 KiB of LDS) with 256 and 512: 134, 146.
+// one of few rows at 128 and 256 elements, or of 8 waves.  More than run at once leave the last
+// ones a CU to themselves: 16 sequences of 1000 to 4000 rows, 32/8 heads, with 256, 512, 1024
+// workgroups: 73, 83, 98 us; 12 tokens each, 16/4 heads of 256, F32 (96 KiB of LDS) with 256
+// and 512: 134, 146.
 void attn_paged_plan(PagedArgs& a, int kv_type, int head_dim, int max_len) {
     const long cap = (long)a.table_ld << a.page_shift;
     const long longest = (max_len < cap ? max_len : cap) + a.max_tok;

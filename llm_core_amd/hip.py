@@ -67,6 +67,10 @@ def _at(p) -> int | None:
 
 
 class Context:
+    """One device and one in-order stream, the context's own: arrays that another stream (torch's)
+    still works on have to be waited for before a call, and the call (sync, download) before
+    that stream reads, writes or frees them."""
+
     def __init__(self, device: int = 0):
         h = C.c_void_p()
         call("axf_hip_create", device, C.byref(h))
