@@ -311,7 +311,8 @@ int axf_hip_kv_fork(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* table_out, in
  * len[s] + i of sequence s.  K row at k + (s * max_tok + i) * k_ld, plus bk, turned
  * (rotate-half RoPE) by row pos[s * max_tok + i] of the tables (cos_t/sin_t
  * [n_pos][head_dim/2], pos clamped to them); pos NULL: not turned.  V row plus
- * bv.  bk, bv may be NULL. */
+ * bv.  bk, bv may be NULL.  The pages written are their sequence's alone
+ * (axf_hip_kv_fork with extra): of two rows at one place either may be left. */
 int axf_hip_kv_store(axf_ctx* ctx, const axf_kv_pages* kv, int layer, const int32_t* table,
                      int table_ld, const int32_t* len, const int32_t* n_tok, int n_seq,
                      int max_tok, const float* k, int k_ld, const float* bk, const float* v,
@@ -360,7 +361,8 @@ int axf_hip_kv_compact(axf_ctx* ctx, const axf_kv_pages* kv, int32_t* len_out,
  * one continuation, eos_id, that keeps its score.  A score of -inf or NaN (a
  * masked token, an unused beam with cum -inf; a row with a NaN or +inf logit) is
  * no continuation.  token, parent (the beam, 0..n_beams-1) and score: n_out a
- * sequence, best first; -1, -1 and -inf where there are no more; with n_out =
+ * sequence, best first; -1, -1 and -inf where there are no more (a continuation's score
+ * below fp32's range comes out as -inf, beside its token and beam); with n_out =
  * n_beams score may be cum.  n_beams and n_out up to 64, n_vocab up to 2^26. */
 int axf_hip_beam_select(axf_ctx* ctx, int32_t* token, int32_t* parent, float* score,
                         const float* logits, int ld, const float* cum, const int32_t* done,

@@ -146,3 +146,25 @@ def test_select_infinite_beam(ctx):
         ctx.beam_select(t, p, s, d.up(x), 700, d.up(cum), 1, 3, 700, 5)
         assert d.get(t, i0)[0].tolist() == np.argsort(-x[0, 1], kind="stable")[:5].tolist()
         assert np.all(d.get(p, i0) == 1) and np.all(d.get(s, f0) == np.inf)
+
+
+def test_select_scores_past_fp32(ctx):
+    """Masks of the type's lowest value, taken twice: the token is there, its score is -inf, and the
+    beam is no candidate in the next step."""
+    low = np.finfo(np.float32).min
+    x = np.full((1, 2, 40), low, np.float32)
+    x[0, 0, 7], x[0, 1, 3] = 0.0, 0.0
+    cum = np.array([[-1.0, low]], np.float32)
+    i0, f0 = np.zeros((1, 2), np.int32), np.zeros((1, 2), np.float32)
+    with R.Device(ctx) as d:
+        t, p, s = d.up(i0), d.up(i0), d.up(cum)
+        lx = d.up(x)
+        ctx.beam_select(t, p, s, lx, 40, s, 1, 2, 40, 2)
+        assert d.get(t, i0).tolist() == [[7, 0]] and d.get(p, i0).tolist() == [[0, 0]]
+        assert d.get(s, f0).tolist() == [[-1.0, low]]
+        one = d.up(np.array([[low, -np.inf]], np.float32))
+        y = d.up(np.full((1, 2, 40), low, np.float32) + np.eye(2, 40, dtype=np.float32)[None] * -low)
+        ctx.beam_select(t, p, s, y, 40, one, 1, 2, 40, 2)
+        # beam 0: its unmasked token, then a masked one at twice the lowest value
+        assert d.get(t, i0).tolist() == [[0, 1]] and d.get(p, i0).tolist() == [[0, 0]]
+        assert d.get(s, f0).tolist() == [[low, -np.inf]]
